@@ -564,6 +564,122 @@ mluOpStatus_t MLUOP_WIN_API mluOpIndiceConvolutionForwardBuiltinWorkspace(
     const int64_t indice_num[], const int64_t num_act_out, const int64_t inverse,
     const int64_t sub_m, const mluOpTensorDescriptor_t features_out_desc, void *features_out);
 
+/* --------------------------------------------- optimiser step, many tensors */
+
+/* No counterpart in the reference with this shape (its mluOpAdamW updates one
+ * tensor, states in float).  One AdamW step over tensor_num tensors at once.
+ * With g = grad * *grad_scale (grad_scale == NULL: 1), t = step:
+ *   m = beta1 * m + (1 - beta1) * g          v = beta2 * v + (1 - beta2) * g * g
+ *   param = param * (1 - lr * weight_decay)
+ *           - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + epsilon)
+ * The arrays element_num[], param[], ... are host arrays of tensor_num entries
+ * (read during the call); what their entries point to lies on the device, dense.
+ *   param_dtype  HALF, BFLOAT16 or FLOAT; the update is computed in float and
+ *                rounded once
+ *   grad_dtype   the same, or FLOAT
+ *   state_dtype  FLOAT: exp_avg[i] and exp_avg_sq[i] hold m and v; the two scale
+ *                arrays are NULL
+ *                UINT8: exp_avg[i] holds m and exp_avg_sq[i] holds sqrt(v), both
+ *                as e4m3 codes (one byte an element), with one float scale per
+ *                256 consecutive elements of the tensor in exp_avg_scale[i] and
+ *                exp_avg_sq_scale[i] (ceil(element_num / 256) floats each): an
+ *                element is code * scale, scale = largest magnitude of the 256 /
+ *                448.  A square root that is not zero is never stored as zero.
+ *                The update itself uses m and v before they are rounded.
+ *                A block whose largest magnitude is below 1e-30 is stored as
+ *                zeros with scale zero.
+ *   schedule     NULL, or three device floats {lr, 1 - beta1^t, 1 - beta2^t} that
+ *                take the place of lr and step and are read when the kernels
+ *                run: what a captured and replayed graph changes from step to
+ *                step.
+ * element_num[i] may be 0 (its pointers are not looked at then).  Requires 0 <=
+ * beta < 1, epsilon >= 0, lr >= 0, step >= 1.  Parameters, gradients and float
+ * states must be aligned to their type; tensors whose pointers are all 16-byte
+ * aligned are moved as 16-byte vectors.  No two tensors may overlap.  A NaN or
+ * infinity in a gradient reaches the elements (8-bit states: the block of 256)
+ * that it belongs to.  Asynchronous on the handle's queue; no workspace. */
+mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW(
+    mluOpHandle_t handle, const mluOpDataType_t param_dtype, const mluOpDataType_t grad_dtype,
+    const mluOpDataType_t state_dtype, const int64_t tensor_num, const int64_t element_num[],
+    void *const param[], const void *const grad[], void *const exp_avg[],
+    void *const exp_avg_sq[], float *const exp_avg_scale[], float *const exp_avg_sq_scale[],
+    const double lr, const double beta1, const double beta2, const double epsilon,
+    const double weight_decay, const int64_t step, const float *grad_scale,
+    const float *schedule);
+
+/* ------------------------------------- group norm with an activation */
+
+/* activation applied to the normalised values */
+typedef enum {
+  MLUOP_GROUP_NORM_ACT_NONE = 0,
+  MLUOP_GROUP_NORM_ACT_RELU = 1,
+  MLUOP_GROUP_NORM_ACT_SILU = 2,
+} mluOpGroupNormAct_t;
+
+/* No counterpart in the reference (this and the three entry points below).
+ * Group norm of channels-last rows with the activation fused.
+ *   input [N, ..., C] (two dimensions or more): sample_ends == NULL, each index
+ *   of the first dimension is a sample; or input [rows, C] with sample_ends [N]
+ *   int32 on the device: sample n is rows sample_ends[n-1] .. sample_ends[n]-1
+ *   (0 before the first), the rows of a sparse tensor's samples one after the
+ *   other.  Entries must not decrease and lie within 0 .. rows (others give
+ *   unspecified outputs, but no access outside of the tensors); samples may be
+ *   empty; rows from the last entry on belong to no sample, their outputs are zero.
+ *   C is a multiple of num_groups.  For sample n and group q:
+ *     mean, var over the sample's rows and the group's channels
+ *     rstd = 1 / sqrt(var + epsilon)
+ *     output = act(weight * (input - mean) * rstd + bias)
+ * input and output HALF, BFLOAT16 or FLOAT, the same; weight and bias [C] FLOAT
+ * or the input's type, both or neither (NULL descriptors: 1 and 0); mean and rstd
+ * [N, num_groups] FLOAT, outputs (an empty sample: mean 0, rstd 1 / sqrt(epsilon)).
+ * epsilon > 0.  Statistics are held in float and combined in a fixed order:
+ * results are reproducible run to run.  Descriptors are contiguous, every tensor
+ * has fewer than 2^31 rows and C <= 65536.  output may be input (in place).
+ * Asynchronous on the handle's queue. */
+mluOpStatus_t MLUOP_WIN_API mluOpGetGroupNormActForwardWorkspaceSize(
+    mluOpHandle_t handle, const mluOpTensorDescriptor_t input_desc,
+    const mluOpTensorDescriptor_t sample_ends_desc, const int64_t num_groups,
+    size_t *workspace_size);
+
+mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActForward(
+    mluOpHandle_t handle, const mluOpTensorDescriptor_t input_desc, const void *input,
+    const mluOpTensorDescriptor_t weight_desc, const void *weight,
+    const mluOpTensorDescriptor_t bias_desc, const void *bias,
+    const mluOpTensorDescriptor_t sample_ends_desc, const void *sample_ends,
+    const int64_t num_groups, const double epsilon, const mluOpGroupNormAct_t activation,
+    void *workspace, const size_t workspace_size, const mluOpTensorDescriptor_t output_desc,
+    void *output, const mluOpTensorDescriptor_t mean_desc, void *mean,
+    const mluOpTensorDescriptor_t rstd_desc, void *rstd);
+
+mluOpStatus_t MLUOP_WIN_API mluOpGetGroupNormActBackwardWorkspaceSize(
+    mluOpHandle_t handle, const mluOpTensorDescriptor_t input_desc,
+    const mluOpTensorDescriptor_t sample_ends_desc, const int64_t num_groups,
+    size_t *workspace_size);
+
+/* Gradients of the above from output_grad and what the forward call read and
+ * wrote (input, weight, bias, mean, rstd; the activation's argument is computed
+ * again).  With xhat = (input - mean) * rstd and du = output_grad * act'(weight *
+ * xhat + bias):
+ *   bias_grad = sum du    weight_grad = sum du * xhat    (over all samples' rows)
+ *   input_grad = rstd * (weight * du - mean(weight * du) - xhat * mean(weight * du * xhat))
+ * (means over the sample's rows and the group's channels).  The gradient of relu
+ * at 0 is 0.  input_grad has the input's type; weight_grad and bias_grad [C]
+ * FLOAT or the input's type, both NULL (descriptors too) to leave them out.
+ * input_grad rows of no sample are zero, and no such row reaches a sum.
+ * input_grad may be output_grad (in place). */
+mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActBackward(
+    mluOpHandle_t handle, const mluOpTensorDescriptor_t output_grad_desc,
+    const void *output_grad, const mluOpTensorDescriptor_t input_desc, const void *input,
+    const mluOpTensorDescriptor_t weight_desc, const void *weight,
+    const mluOpTensorDescriptor_t bias_desc, const void *bias,
+    const mluOpTensorDescriptor_t sample_ends_desc, const void *sample_ends,
+    const mluOpTensorDescriptor_t mean_desc, const void *mean,
+    const mluOpTensorDescriptor_t rstd_desc, const void *rstd, const int64_t num_groups,
+    const mluOpGroupNormAct_t activation, void *workspace, const size_t workspace_size,
+    const mluOpTensorDescriptor_t input_grad_desc, void *input_grad,
+    const mluOpTensorDescriptor_t weight_grad_desc, void *weight_grad,
+    const mluOpTensorDescriptor_t bias_grad_desc, void *bias_grad);
+
 #if defined(__cplusplus)
 }
 #endif

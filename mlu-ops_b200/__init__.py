@@ -7,6 +7,7 @@ follow the reference's C API.  There is no CPU fallback: if the library has not
 been built, loading raises.
 """
 import ctypes
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -27,6 +28,9 @@ STATUS_NUMERICAL_OVERFLOW = 8
 LAYOUT_NCHW, LAYOUT_NHWC, LAYOUT_HWCN, LAYOUT_NDHWC, LAYOUT_ARRAY, LAYOUT_NCDHW = 0, 1, 2, 3, 4, 5
 # mluOpDataType_t
 DTYPE_INVALID, DTYPE_HALF, DTYPE_FLOAT, DTYPE_INT16, DTYPE_INT32, DTYPE_INT64 = 0, 1, 2, 4, 6, 9
+DTYPE_UINT8, DTYPE_BFLOAT16 = 7, 17
+# mluOpGroupNormAct_t
+GROUP_NORM_ACTS = {"none": 0, "relu": 1, "silu": 2}
 
 _vp = ctypes.c_void_p
 _int = ctypes.c_int
@@ -109,6 +113,11 @@ SIGNATURES = {
                                                                ctypes.POINTER(_szt)]),
     "mluOpDynamicPointToVoxelBackward": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                                _vp, _szt, _vp, _vp]),
+    "mluOpMultiTensorAdamW": (_int, [_vp, _int, _int, _int, _i64] + [_vp] * 7 + [ctypes.c_double] * 5 + [_i64, _vp, _vp]),
+    "mluOpGetGroupNormActForwardWorkspaceSize": (_int, [_vp, _vp, _vp, _i64, ctypes.POINTER(_szt)]),
+    "mluOpGroupNormActForward": (_int, [_vp] * 9 + [_i64, ctypes.c_double, _int, _vp, _szt] + [_vp] * 6),
+    "mluOpGetGroupNormActBackwardWorkspaceSize": (_int, [_vp, _vp, _vp, _i64, ctypes.POINTER(_szt)]),
+    "mluOpGroupNormActBackward": (_int, [_vp] * 15 + [_i64, _int, _vp, _szt] + [_vp] * 6),
     # include/mlu_op_trace.h
     "mluOpTraceKernelEnable": (_int, [_int]),
     "mluOpTraceKernelReset": (_int, []),
@@ -160,6 +169,9 @@ class Handle:
     def __init__(self, stream=0):
         self.ptr = _vp()
         check("mluOpCreate", lib().mluOpCreate(ctypes.byref(self.ptr)))
+        device = ctypes.c_int(-1)
+        check("mluOpGetDevice", lib().mluOpGetDevice(self.ptr, ctypes.byref(device)))
+        self.device = device.value  # CUDA device ordinal, -1 for a host-only handle
         self.set_queue(stream)
 
     def set_queue(self, stream):
@@ -186,6 +198,7 @@ class TensorDesc:
         check("mluOpSetTensorDescriptor_v2",
               lib().mluOpSetTensorDescriptor_v2(self.ptr, layout, dtype, len(dims), i64_array(dims)))
         self.dims = tuple(int(d) for d in dims)
+        self._as_parameter_ = self.ptr  # a call may be given the object itself, which then outlives it
 
     def destroy(self):
         if self.ptr:
@@ -723,3 +736,199 @@ def dynamic_point_to_voxel_backward(handle, grad_voxel_feats, feats, voxel_feats
     for d in descs:
         d.destroy()
     return grad_feats
+
+
+# ---------------------------------------------------------------- operators of a training step
+
+
+@functools.lru_cache(maxsize=1024)
+def _array_desc(dtype, dims):
+    """A contiguous descriptor, shared by the calls that describe a tensor of this type and shape."""
+    return TensorDesc(LAYOUT_ARRAY, dtype, dims)
+
+
+_dtype_codes = {}
+
+
+def _dtype_code(torch_dtype):
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({torch.float16: DTYPE_HALF, torch.bfloat16: DTYPE_BFLOAT16, torch.float32: DTYPE_FLOAT,
+                             torch.int32: DTYPE_INT32, torch.int64: DTYPE_INT64, torch.uint8: DTYPE_UINT8,
+                             torch.float8_e4m3fn: DTYPE_UINT8})
+    return _dtype_codes.get(torch_dtype, DTYPE_INVALID)
+
+
+def _desc_of(handle, name, t):
+    """Descriptor of tensor `t`, which must lie densely on the handle's device; (None, None) without one."""
+    if t is None:
+        return None, None
+    if t.get_device() != handle.device:
+        raise ValueError("%s lies on %s, the handle on CUDA device %d" % (name, t.device, handle.device))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    return _array_desc(_dtype_code(t.dtype), tuple(t.shape)), _vp(t.data_ptr())
+
+
+def _group_norm_workspace(handle, query, d_input, d_ends, num_groups, device):
+    import torch
+    size = _szt(0)
+    check(query, getattr(lib(), query)(handle.ptr, d_input, d_ends, num_groups, ctypes.byref(size)))
+    return _alloc((size.value,), torch.uint8, device), size.value
+
+
+def group_norm_act_forward(handle, input, weight, bias, num_groups, epsilon=1e-5, activation="none", sample_ends=None,
+                           out=None):
+    """Group norm of channels-last rows with an activation ("none", "relu", "silu") through
+    mluOpGroupNormActForward.
+
+    input [N, ..., C] with a sample for each index of the first dimension, or [rows, C] with
+    sample_ends, int32 [N]: where each sample's rows end (rows behind the last end: zeros out).
+    weight and bias [C] (float32 or input's type) or both None.  Returns (output, mean, rstd),
+    mean and rstd float32 [N, num_groups].  out: the output tensor, may be input.
+    """
+    import torch
+    if activation not in GROUP_NORM_ACTS:
+        raise ValueError("activation is one of %s" % ", ".join(GROUP_NORM_ACTS))
+    d_x, p_x = _desc_of(handle, "input", input)
+    d_w, p_w = _desc_of(handle, "weight", weight)
+    d_b, p_b = _desc_of(handle, "bias", bias)
+    d_e, p_e = _desc_of(handle, "sample_ends", sample_ends)
+    num_groups = int(num_groups)
+    workspace, size = _group_norm_workspace(handle, "mluOpGetGroupNormActForwardWorkspaceSize", d_x, d_e, num_groups,
+                                            input.device)
+    samples = input.shape[0] if sample_ends is None else sample_ends.shape[0]
+    if out is None:
+        out = _alloc(input.shape, input.dtype, input.device)
+    mean = _alloc((samples, num_groups), torch.float32, input.device)
+    rstd = _alloc((samples, num_groups), torch.float32, input.device)
+    d_y, p_y = _desc_of(handle, "out", out)
+    d_m = _array_desc(DTYPE_FLOAT, (samples, num_groups))
+    check("mluOpGroupNormActForward",
+          lib().mluOpGroupNormActForward(handle.ptr, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, num_groups, epsilon,
+                                         GROUP_NORM_ACTS[activation], _ptr(workspace), size, d_y, p_y, d_m, _ptr(mean),
+                                         d_m, _ptr(rstd)))
+    return out, mean, rstd
+
+
+def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd, num_groups, activation="none",
+                            sample_ends=None, affine_grad=True, affine_grad_dtype=None, out=None):
+    """(input_grad, weight_grad, bias_grad) of group_norm_act_forward through mluOpGroupNormActBackward.
+
+    mean and rstd are the forward call's; affine_grad=False leaves the two affine gradients out
+    (None); affine_grad_dtype: float32 (default) or input's type.  out: the input gradient's
+    tensor, may be output_grad.
+    """
+    import torch
+    if activation not in GROUP_NORM_ACTS:
+        raise ValueError("activation is one of %s" % ", ".join(GROUP_NORM_ACTS))
+    d_g, p_g = _desc_of(handle, "output_grad", output_grad)
+    d_x, p_x = _desc_of(handle, "input", input)
+    d_w, p_w = _desc_of(handle, "weight", weight)
+    d_b, p_b = _desc_of(handle, "bias", bias)
+    d_e, p_e = _desc_of(handle, "sample_ends", sample_ends)
+    d_m, p_m = _desc_of(handle, "mean", mean)
+    d_r, p_r = _desc_of(handle, "rstd", rstd)
+    num_groups = int(num_groups)
+    workspace, size = _group_norm_workspace(handle, "mluOpGetGroupNormActBackwardWorkspaceSize", d_x, d_e, num_groups,
+                                            input.device)
+    if out is None:
+        out = _alloc(input.shape, input.dtype, input.device)
+    d_o, p_o = _desc_of(handle, "out", out)
+    weight_grad = bias_grad = None
+    if affine_grad:
+        weight_grad = _alloc((input.shape[-1],), affine_grad_dtype or torch.float32, input.device)
+        bias_grad = _alloc((input.shape[-1],), affine_grad_dtype or torch.float32, input.device)
+    d_wg, p_wg = _desc_of(handle, "weight_grad", weight_grad)
+    d_bg, p_bg = _desc_of(handle, "bias_grad", bias_grad)
+    check("mluOpGroupNormActBackward",
+          lib().mluOpGroupNormActBackward(handle.ptr, d_g, p_g, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, d_m, p_m, d_r,
+                                          p_r, num_groups, GROUP_NORM_ACTS[activation], _ptr(workspace), size, d_o,
+                                          p_o, d_wg, p_wg, d_bg, p_bg))
+    return out, weight_grad, bias_grad
+
+
+SCALE_BLOCK = 256  # consecutive elements of an 8-bit optimiser state that share a scale
+
+
+def _addresses(tensors):
+    return (_vp * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+class MultiTensorAdamW:
+    """AdamW steps over the same tensors through mluOpMultiTensorAdamW.
+
+    params: dense CUDA tensors of one type (float32, float16 or bfloat16), updated in place;
+    exp_avgs and exp_avg_sqs: their states, of the same element counts.  float32 states hold the
+    moments themselves.  8-bit states (uint8 or float8_e4m3fn) hold the first moment and the
+    square root of the second as e4m3 codes; exp_avg_scales and exp_avg_sq_scales then hold one
+    float32 for each 256 elements of their tensor (code * scale is the value).  The object keeps
+    references to the tensors, whose storage has to stay where it is between the steps.
+    """
+
+    def __init__(self, params, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_avg_sq_scales=None):
+        import torch
+        self.params, self.exp_avgs, self.exp_avg_sqs = list(params), list(exp_avgs), list(exp_avg_sqs)
+        if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
+            raise ValueError("the scales of both states come together")
+        self.eight_bit = exp_avg_scales is not None
+        self.scales = [list(exp_avg_scales), list(exp_avg_sq_scales)] if self.eight_bit else []
+        if any(len(v) != len(self.params) for v in [self.exp_avgs, self.exp_avg_sqs] + self.scales):
+            raise ValueError("the lists have different lengths")
+        self.numels = [p.numel() for p in self.params]
+        self.dtype = self.params[0].dtype if self.params else torch.float32
+        self.device = self.params[0].get_device() if self.params else None
+        states = (torch.uint8, torch.float8_e4m3fn) if self.eight_bit else (torch.float32,)
+        spans = []
+        for p, m, v, n in zip(self.params, self.exp_avgs, self.exp_avg_sqs, self.numels):
+            if p.dtype != self.dtype or m.dtype not in states or v.dtype not in states:
+                raise ValueError("parameters have one type, states are float32, or 8 bits with scales")
+            if m.numel() != n or v.numel() != n:
+                raise ValueError("a state has another number of elements than its parameter")
+            spans += [p, m, v]
+        for scales in self.scales:
+            for q, n in zip(scales, self.numels):
+                if q.dtype != torch.float32 or q.numel() != -(-n // SCALE_BLOCK):
+                    raise ValueError("scales are float32, one for each %d elements" % SCALE_BLOCK)
+                spans.append(q)
+        end = 0
+        for begin, size, t in sorted(((t.data_ptr(), t.numel() * t.element_size(), t) for t in spans),
+                                     key=lambda x: x[:2]):
+            if t.get_device() != self.device or not t.is_contiguous():
+                raise ValueError("every tensor is dense and on the same device")
+            if size and begin < end:
+                raise ValueError("two of the tensors overlap")
+            end = max(end, begin + size)
+        self._param_p, self._m_p, self._v_p = _addresses(self.params), _addresses(self.exp_avgs), _addresses(self.exp_avg_sqs)
+        self._scale_p = [_addresses(v) for v in self.scales] or [None, None]
+        self._numel_p = i64_array(self.numels)
+
+    def step(self, handle, grads, lr, betas=(0.9, 0.999), epsilon=1e-8, weight_decay=0.01, step=1, grad_scale=None,
+             schedule=None):
+        """One step with the gradients `grads` (dense, in the parameters' order; their type or float32).
+
+        step counts from 1.  grad_scale: a float32 CUDA tensor of one element that every gradient is
+        multiplied by (a clipping or loss-scale factor).  schedule: a float32 CUDA tensor {lr,
+        1 - beta1^step, 1 - beta2^step} that takes the place of lr and step when the kernels run.
+        """
+        import torch
+        if len(grads) != len(self.params):
+            raise ValueError("%d gradients for %d parameters" % (len(grads), len(self.params)))
+        if not grads:
+            return
+        if self.device != handle.device:
+            raise ValueError("the tensors lie on device %s, the handle on CUDA device %d" % (self.device, handle.device))
+        dtype = grads[0].dtype
+        for g, n in zip(grads, self.numels):
+            if g.dtype is not dtype or g.numel() != n or g.get_device() != self.device or not g.is_contiguous():
+                raise ValueError("gradients are dense, of one type, on the parameters' device and of their sizes")
+        for name, t, n in (("grad_scale", grad_scale, 1), ("schedule", schedule, 3)):
+            if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.get_device() != self.device
+                                  or not t.is_contiguous()):
+                raise ValueError("%s is a dense float32 tensor of %d element(s) on the parameters' device" % (name, n))
+        check("mluOpMultiTensorAdamW",
+              lib().mluOpMultiTensorAdamW(handle.ptr, _dtype_code(self.dtype), _dtype_code(dtype),
+                                          DTYPE_UINT8 if self.eight_bit else DTYPE_FLOAT, len(self.params),
+                                          self._numel_p, self._param_p, _addresses(grads), self._m_p, self._v_p,
+                                          *self._scale_p, lr, betas[0], betas[1], epsilon, weight_decay, int(step),
+                                          _ptr(grad_scale), _ptr(schedule)))

@@ -1,11 +1,12 @@
 """Builds libmluops_b200.so: the C-ABI library with the sm_100a kernels.
 
-One nvcc invocation over the C++ host sources and the CUDA kernels; the output
-is placed next to this file under lib/ (git-ignored, shipped as a built
-artefact).  nvcc cross-compiles, so no GPU is needed to build.
+One nvcc invocation for each C++ host source and CUDA file, then one that links
+them; the output is placed next to this file under lib/ (git-ignored, shipped as
+a built artefact).  nvcc cross-compiles, so no GPU is needed to build.
 
 Usage: python mlu-ops_b200/build.py [--force] [--verbose]
 """
+import concurrent.futures
 import glob
 import os
 import subprocess
@@ -15,23 +16,28 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
+OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB = os.path.join(LIB_DIR, "libmluops_b200.so")
 
 
+KERNEL_DIRS = ("sparse_conv", "voxelization", "dynamic_point_to_voxel", "multi_tensor_adamw", "group_norm_act",
+               "grouped_matmul")
+
+
 def sources():
-    out = []
-    for pattern in ("core/*.cpp", "kernels/sparse_conv/*.cpp", "kernels/sparse_conv/*.cu",
-                    "kernels/voxelization/*.cpp", "kernels/voxelization/*.cu",
-                    "kernels/dynamic_point_to_voxel/*.cpp", "kernels/dynamic_point_to_voxel/*.cu"):
-        out += sorted(glob.glob(os.path.join(CSRC, pattern)))
+    out = sorted(glob.glob(os.path.join(CSRC, "core", "*.cpp")))
+    for d in KERNEL_DIRS:
+        for pattern in ("*.cpp", "*.cu"):
+            out += sorted(glob.glob(os.path.join(CSRC, "kernels", d, pattern)))
     return out
 
 
 def headers():
-    out = glob.glob(os.path.join(ROOT, "include", "*.h"))
-    for pattern in ("core/*.h", "kernels/sparse_conv/*.h", "kernels/sparse_conv/*.cuh", "kernels/voxelization/*.h",
-                    "kernels/dynamic_point_to_voxel/*.h"):
-        out += glob.glob(os.path.join(CSRC, pattern))
+    out = (glob.glob(os.path.join(ROOT, "include", "*.h")) + glob.glob(os.path.join(CSRC, "core", "*.h"))
+           + glob.glob(os.path.join(CSRC, "core", "*.cuh")))
+    for d in KERNEL_DIRS:
+        for pattern in ("*.h", "*.cuh"):
+            out += glob.glob(os.path.join(CSRC, "kernels", d, pattern))
     return out
 
 
@@ -39,16 +45,16 @@ def up_to_date():
     if not os.path.isfile(LIB):
         return False
     t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(p) <= t for p in sources() + headers())
+    return all(os.path.getmtime(p) <= t for p in sources() + headers() + [os.path.abspath(__file__)])
 
 
 def build(force=False, verbose=False):
     if not force and up_to_date():
         return LIB
-    os.makedirs(LIB_DIR, exist_ok=True)
+    os.makedirs(OBJ_DIR, exist_ok=True)
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    cmd = [
-        nvcc, "-shared", "-o", LIB, "-std=c++17", "-O3", "-lineinfo",
+    flags = [
+        "-std=c++17", "-O3", "-lineinfo",
         "-gencode", "arch=compute_100a,code=sm_100a",
         "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall",
         "-DMLUOP_WIN_API=__attribute__((visibility(\"default\")))",
@@ -56,13 +62,31 @@ def build(force=False, verbose=False):
         "-I", os.path.join(ROOT, "include"), "-I", CSRC,
     ]
     if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += os.environ.get("MLUOP_B200_NVCC_FLAGS", "").split()  # extra compiler flags (experiments)
-    cmd += sources()
-    cmd += ["-lcudart_static", "-lpthread", "-ldl", "-lrt"]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
+        flags += ["-Xptxas", "-v"]
+    flags += os.environ.get("MLUOP_B200_NVCC_FLAGS", "").split()  # extra compiler flags (experiments)
+
+    # One object per source, compiled side by side; an object is kept while its own source, every
+    # header and the flags are older than it.
+    flag_file = os.path.join(OBJ_DIR, "flags.txt")
+    same_flags = os.path.isfile(flag_file) and open(flag_file).read() == " ".join([nvcc] + flags)
+    newest_header = max(os.path.getmtime(p) for p in headers())
+
+    def compile_one(src):
+        obj = os.path.join(OBJ_DIR, os.path.relpath(src, CSRC).replace(os.sep, "__") + ".o")
+        if (force or not same_flags or not os.path.isfile(obj)
+                or os.path.getmtime(obj) < max(os.path.getmtime(src), newest_header)):
+            cmd = [nvcc, "-c", "-o", obj] + flags + [src]
+            if verbose:
+                print(" ".join(cmd))
+            subprocess.check_call(cmd)
+        return obj
+
+    with concurrent.futures.ThreadPoolExecutor(os.cpu_count()) as pool:
+        objects = list(pool.map(compile_one, sources()))
+    with open(flag_file, "w") as f:
+        f.write(" ".join([nvcc] + flags))
+    subprocess.check_call([nvcc, "-shared", "-o", LIB, "-gencode", "arch=compute_100a,code=sm_100a"] + objects
+                          + ["-lcudart_static", "-lpthread", "-ldl", "-lrt"])
     return LIB
 
 

@@ -29,6 +29,16 @@ bool takeStickyDeviceError(mluOpHandle_t handle, const char *api) {
   return true;
 }
 
+DeviceGuard::DeviceGuard(mluOpHandle_t handle) {
+  int current = -1;
+  if (handle->host_only || cudaGetDevice(&current) != cudaSuccess || current == handle->device) return;
+  if (cudaSetDevice(handle->device) == cudaSuccess) previous_ = current;
+}
+
+DeviceGuard::~DeviceGuard() {
+  if (previous_ >= 0) cudaSetDevice(previous_);
+}
+
 }  // namespace mluop
 
 extern "C" {

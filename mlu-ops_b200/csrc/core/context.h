@@ -63,6 +63,19 @@ bool checkStatusRequested();
 // synchronisation: only errors that have already reached the host are seen.
 bool takeStickyDeviceError(mluOpHandle_t handle, const char *api);
 
+// Makes the handle's device the current one for the guard's lifetime, so that a call works whichever
+// device the calling thread has selected.
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(mluOpHandle_t handle);
+  ~DeviceGuard();
+  DeviceGuard(const DeviceGuard &) = delete;
+  DeviceGuard &operator=(const DeviceGuard &) = delete;
+
+ private:
+  int previous_ = -1;  // device to go back to, -1: nothing was changed
+};
+
 }  // namespace mluop
 
 #endif  // MLUOP_B200_CORE_CONTEXT_H_
