@@ -680,6 +680,54 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActBackward(
     const mluOpTensorDescriptor_t weight_grad_desc, void *weight_grad,
     const mluOpTensorDescriptor_t bias_grad_desc, void *bias_grad);
 
+/* ------------------------------------- matrix products grouped by row blocks */
+
+/* No counterpart in the reference (this and the three entry points below).  The
+ * rows of a matrix lie grouped: group g is rows group_ends[g-1] ..
+ * group_ends[g]-1 (0 before the first), and has a matrix of its own:
+ *   output[r,:] = input[r,:] * weight[g,:,:]      for the rows r of group g
+ * input [rows,Ci], weight [G,Ci,Co] (the convolution's ARRAY order), group_ends
+ * [G] int32 on the device, output [rows,Co]; HALF, BFLOAT16 or FLOAT, all three
+ * the same; accumulation in float.  The row counts stay on the device: nothing
+ * is read back, and a captured graph follows them.  Entries of group_ends are
+ * clamped to [previous entry, rows]; groups may be empty; rows from the last
+ * entry on belong to no group and their outputs are zero.  1 <= G <= 1024, rows <
+ * 2^31, 1 <= Ci, Co <= 65536, and fewer than 2^30 tiles of 128 x 64 results.  HALF and BFLOAT16 run on the tensor cores where Ci
+ * and Co are multiples of 8 and the three pointers are 16-byte aligned, else on the
+ * general kernel.  Outputs may not overlap inputs.  Results are reproducible run
+ * to run.  Asynchronous on the handle's queue; no workspace. */
+mluOpStatus_t MLUOP_WIN_API mluOpGroupedMatMulForward(
+    mluOpHandle_t handle, const mluOpTensorDescriptor_t input_desc, const void *input,
+    const mluOpTensorDescriptor_t weight_desc, const void *weight,
+    const mluOpTensorDescriptor_t group_ends_desc, const void *group_ends,
+    const mluOpTensorDescriptor_t output_desc, void *output);
+
+/*   input_grad[r,:] = output_grad[r,:] * weight[g,:,:]^T
+ * under the same terms. */
+mluOpStatus_t MLUOP_WIN_API mluOpGroupedMatMulBackwardInput(
+    mluOpHandle_t handle, const mluOpTensorDescriptor_t output_grad_desc,
+    const void *output_grad, const mluOpTensorDescriptor_t weight_desc, const void *weight,
+    const mluOpTensorDescriptor_t group_ends_desc, const void *group_ends,
+    const mluOpTensorDescriptor_t input_grad_desc, void *input_grad);
+
+/* Device scratch of the weight gradient: float partial sums where a group's rows
+ * are split over several blocks, 160 MB at most, and 256 bytes a group. */
+mluOpStatus_t MLUOP_WIN_API mluOpGetGroupedMatMulBackwardWeightWorkspaceSize(
+    mluOpHandle_t handle, const mluOpTensorDescriptor_t input_desc,
+    const mluOpTensorDescriptor_t output_grad_desc,
+    const mluOpTensorDescriptor_t weight_grad_desc, size_t *workspace_size);
+
+/*   weight_grad[g,:,:] = sum over the rows r of group g of input[r,:]^T output_grad[r,:]
+ * input [rows,Ci], output_grad [rows,Co] the same type; weight_grad [G,Ci,Co] that
+ * type or FLOAT.  An empty group's gradient is zero; rows of no group take no part,
+ * whatever they hold. */
+mluOpStatus_t MLUOP_WIN_API mluOpGroupedMatMulBackwardWeight(
+    mluOpHandle_t handle, const mluOpTensorDescriptor_t input_desc, const void *input,
+    const mluOpTensorDescriptor_t output_grad_desc, const void *output_grad,
+    const mluOpTensorDescriptor_t group_ends_desc, const void *group_ends, void *workspace,
+    const size_t workspace_size, const mluOpTensorDescriptor_t weight_grad_desc,
+    void *weight_grad);
+
 #if defined(__cplusplus)
 }
 #endif

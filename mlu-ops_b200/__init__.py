@@ -118,6 +118,10 @@ SIGNATURES = {
     "mluOpGroupNormActForward": (_int, [_vp] * 9 + [_i64, ctypes.c_double, _int, _vp, _szt] + [_vp] * 6),
     "mluOpGetGroupNormActBackwardWorkspaceSize": (_int, [_vp, _vp, _vp, _i64, ctypes.POINTER(_szt)]),
     "mluOpGroupNormActBackward": (_int, [_vp] * 15 + [_i64, _int, _vp, _szt] + [_vp] * 6),
+    "mluOpGroupedMatMulForward": (_int, [_vp] * 9),
+    "mluOpGroupedMatMulBackwardInput": (_int, [_vp] * 9),
+    "mluOpGetGroupedMatMulBackwardWeightWorkspaceSize": (_int, [_vp, _vp, _vp, _vp, ctypes.POINTER(_szt)]),
+    "mluOpGroupedMatMulBackwardWeight": (_int, [_vp] * 8 + [_szt, _vp, _vp]),
     # include/mlu_op_trace.h
     "mluOpTraceKernelEnable": (_int, [_int]),
     "mluOpTraceKernelReset": (_int, []),
@@ -932,3 +936,57 @@ class MultiTensorAdamW:
                                           self._numel_p, self._param_p, _addresses(grads), self._m_p, self._v_p,
                                           *self._scale_p, lr, betas[0], betas[1], epsilon, weight_decay, int(step),
                                           _ptr(grad_scale), _ptr(schedule)))
+
+
+def grouped_matmul_forward(handle, input, weight, group_ends, out=None):
+    """output [rows,Co] with output[r] = input[r] @ weight[g] for the rows r of group g, through
+    mluOpGroupedMatMulForward.
+
+    input [rows,Ci], weight [G,Ci,Co] of one type (float16, bfloat16, float32); group_ends int32
+    [G] on the device: group g's rows end there, the next group's begin.  Rows behind the last
+    group's end: zeros.
+    """
+    d_x, p_x = _desc_of(handle, "input", input)
+    d_w, p_w = _desc_of(handle, "weight", weight)
+    d_e, p_e = _desc_of(handle, "group_ends", group_ends)
+    if out is None:
+        out = _alloc((input.shape[0], weight.shape[-1]), input.dtype, input.device)
+    d_y, p_y = _desc_of(handle, "out", out)
+    check("mluOpGroupedMatMulForward",
+          lib().mluOpGroupedMatMulForward(handle.ptr, d_x, p_x, d_w, p_w, d_e, p_e, d_y, p_y))
+    return out
+
+
+def grouped_matmul_backward_input(handle, output_grad, weight, group_ends, out=None):
+    """input_grad [rows,Ci] with input_grad[r] = output_grad[r] @ weight[g].T through
+    mluOpGroupedMatMulBackwardInput (the forward call's arguments)."""
+    d_g, p_g = _desc_of(handle, "output_grad", output_grad)
+    d_w, p_w = _desc_of(handle, "weight", weight)
+    d_e, p_e = _desc_of(handle, "group_ends", group_ends)
+    if out is None:
+        out = _alloc((output_grad.shape[0], weight.shape[-2]), output_grad.dtype, output_grad.device)
+    d_x, p_x = _desc_of(handle, "out", out)
+    check("mluOpGroupedMatMulBackwardInput",
+          lib().mluOpGroupedMatMulBackwardInput(handle.ptr, d_g, p_g, d_w, p_w, d_e, p_e, d_x, p_x))
+    return out
+
+
+def grouped_matmul_backward_weight(handle, input, output_grad, group_ends, dtype=None, workspace=None, out=None):
+    """weight_grad [G,Ci,Co] with weight_grad[g] = input[rows of g].T @ output_grad[rows of g] through
+    mluOpGroupedMatMulBackwardWeight; dtype: input's (default) or float32."""
+    import torch
+    d_x, p_x = _desc_of(handle, "input", input)
+    d_g, p_g = _desc_of(handle, "output_grad", output_grad)
+    d_e, p_e = _desc_of(handle, "group_ends", group_ends)
+    if out is None:
+        out = _alloc((group_ends.shape[0], input.shape[-1], output_grad.shape[-1]), dtype or input.dtype, input.device)
+    d_w, p_w = _desc_of(handle, "out", out)
+    size = _szt(0)
+    check("mluOpGetGroupedMatMulBackwardWeightWorkspaceSize",
+          lib().mluOpGetGroupedMatMulBackwardWeightWorkspaceSize(handle.ptr, d_x, d_g, d_w, ctypes.byref(size)))
+    if workspace is None or workspace.numel() < size.value:
+        workspace = _alloc((size.value,), torch.uint8, input.device)
+    check("mluOpGroupedMatMulBackwardWeight",
+          lib().mluOpGroupedMatMulBackwardWeight(handle.ptr, d_x, p_x, d_g, p_g, d_e, p_e, _ptr(workspace), size.value,
+                                                 d_w, p_w))
+    return out

@@ -24,8 +24,8 @@ bool takeStickyDeviceError(mluOpHandle_t handle, const char *api) {
   if (bits == 0) return false;
   *word = 0;
   LOG(ERROR) << api << " an earlier asynchronous call on this handle reported device error bits " << bits
-             << " (1: hash table full, 4: look-back wait gave up, 0x100 and up: a bounded wait of the "
-             << "convolution kernel gave up); its outputs are not valid.";
+             << " (1: hash table full, 4: look-back wait gave up, 0x100 and up: a bounded wait of a "
+             << "tensor-core kernel gave up); its outputs are not valid.";
   return true;
 }
 

@@ -34,11 +34,11 @@ __device__ __forceinline__ bool mbarTryWait(unsigned long long *bar, unsigned pa
   return ok != 0;
 }
 struct ErrorSink {
-  int32_t *status;  // status word in the workspace
+  int32_t *status;  // status word in the workspace, or null
   int32_t *sticky;  // device-visible host word of the handle, or null
 };
 __device__ __forceinline__ void raiseWaitError(const ErrorSink &sink, int code) {
-  atomicOr(sink.status, code);
+  if (sink.status) atomicOr(sink.status, code);
   if (sink.sticky) {
     *reinterpret_cast<volatile int32_t *>(sink.sticky) = code << 8;
     __threadfence_system();
