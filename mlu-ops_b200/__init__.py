@@ -7,7 +7,6 @@ follow the reference's C API.  There is no CPU fallback: if the library has not
 been built, loading raises.
 """
 import ctypes
-import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -176,6 +175,7 @@ class Handle:
         device = ctypes.c_int(-1)
         check("mluOpGetDevice", lib().mluOpGetDevice(self.ptr, ctypes.byref(device)))
         self.device = device.value  # CUDA device ordinal, -1 for a host-only handle
+        self.plans = {}  # descriptors and workspace sizes of the calls seen, by types and shapes
         self.set_queue(stream)
 
     def set_queue(self, stream):
@@ -202,7 +202,7 @@ class TensorDesc:
         check("mluOpSetTensorDescriptor_v2",
               lib().mluOpSetTensorDescriptor_v2(self.ptr, layout, dtype, len(dims), i64_array(dims)))
         self.dims = tuple(int(d) for d in dims)
-        self._as_parameter_ = self.ptr  # a call may be given the object itself, which then outlives it
+        self._as_parameter_ = self.ptr  # the object itself can be handed to a call
 
     def destroy(self):
         if self.ptr:
@@ -743,13 +743,10 @@ def dynamic_point_to_voxel_backward(handle, grad_voxel_feats, feats, voxel_feats
 
 
 # ---------------------------------------------------------------- operators of a training step
-
-
-@functools.lru_cache(maxsize=1024)
-def _array_desc(dtype, dims):
-    """A contiguous descriptor, shared by the calls that describe a tensor of this type and shape."""
-    return TensorDesc(LAYOUT_ARRAY, dtype, dims)
-
+#
+# A call of these operators checks its tensors, then finds the descriptors and the workspace size
+# for their types and shapes in a table that its handle keeps: building them anew would take longer
+# than a small operator runs.
 
 _dtype_codes = {}
 
@@ -763,22 +760,60 @@ def _dtype_code(torch_dtype):
     return _dtype_codes.get(torch_dtype, DTYPE_INVALID)
 
 
-def _desc_of(handle, name, t):
-    """Descriptor of tensor `t`, which must lie densely on the handle's device; (None, None) without one."""
-    if t is None:
-        return None, None
+def _address(handle, name, t):
+    """The address of tensor `t`, which must lie densely on the handle's device."""
     if t.get_device() != handle.device:
         raise ValueError("%s lies on %s, the handle on CUDA device %d" % (name, t.device, handle.device))
     if not t.is_contiguous():
         raise ValueError("%s must be contiguous" % name)
-    return _array_desc(_dtype_code(t.dtype), tuple(t.shape)), _vp(t.data_ptr())
+    return t.data_ptr()
 
 
-def _group_norm_workspace(handle, query, d_input, d_ends, num_groups, device):
+class _CallPlan:
+    """Descriptors (d: their addresses, in the order of `specs`; None stays None) and workspace bytes of a call."""
+    __slots__ = ("descs", "d", "workspace")
+
+    def __init__(self, specs):
+        self.descs = [None if s is None else TensorDesc(LAYOUT_ARRAY, _dtype_code(s[0]), tuple(s[1])) for s in specs]
+        self.d = [None if t is None else t.ptr.value for t in self.descs]
+        self.workspace = 0
+
+
+def _call_plan(handle, key, specs, query=None):
+    """The handle's plan for `key`; a new one describes `specs()` and asks `query(plan, size)` for its workspace."""
+    plan = handle.plans.get(key)
+    if plan is None:
+        plan = _CallPlan(specs())
+        if query is not None:
+            size = _szt(0)
+            query(plan, size)
+            plan.workspace = size.value
+        if len(handle.plans) >= 512:  # shapes that change from step to step do not pile up
+            handle.plans.clear()
+        handle.plans[key] = plan
+    return plan
+
+
+def _new(like, shape, dtype):
+    if _guards is not None:
+        return _guards.empty(shape, dtype, like.device)
+    return like.new_empty(shape, dtype=dtype)
+
+
+def _workspace(like, nbytes):
     import torch
-    size = _szt(0)
-    check(query, getattr(lib(), query)(handle.ptr, d_input, d_ends, num_groups, ctypes.byref(size)))
-    return _alloc((size.value,), torch.uint8, device), size.value
+    return _new(like, (nbytes,), torch.uint8)
+
+
+def _spec(t):
+    return None if t is None else (t.dtype, t.shape)
+
+
+def _activation(name):
+    code = GROUP_NORM_ACTS.get(name)
+    if code is None:
+        raise ValueError("activation is one of %s" % ", ".join(GROUP_NORM_ACTS))
+    return code
 
 
 def group_norm_act_forward(handle, input, weight, bias, num_groups, epsilon=1e-5, activation="none", sample_ends=None,
@@ -792,26 +827,29 @@ def group_norm_act_forward(handle, input, weight, bias, num_groups, epsilon=1e-5
     mean and rstd float32 [N, num_groups].  out: the output tensor, may be input.
     """
     import torch
-    if activation not in GROUP_NORM_ACTS:
-        raise ValueError("activation is one of %s" % ", ".join(GROUP_NORM_ACTS))
-    d_x, p_x = _desc_of(handle, "input", input)
-    d_w, p_w = _desc_of(handle, "weight", weight)
-    d_b, p_b = _desc_of(handle, "bias", bias)
-    d_e, p_e = _desc_of(handle, "sample_ends", sample_ends)
+    act = _activation(activation)
+    p_x = _address(handle, "input", input)
+    p_w = None if weight is None else _address(handle, "weight", weight)
+    p_b = None if bias is None else _address(handle, "bias", bias)
+    p_e = None if sample_ends is None else _address(handle, "sample_ends", sample_ends)
     num_groups = int(num_groups)
-    workspace, size = _group_norm_workspace(handle, "mluOpGetGroupNormActForwardWorkspaceSize", d_x, d_e, num_groups,
-                                            input.device)
-    samples = input.shape[0] if sample_ends is None else sample_ends.shape[0]
+    stats = ((input.shape[0] if sample_ends is None else sample_ends.shape[0]), num_groups)
     if out is None:
-        out = _alloc(input.shape, input.dtype, input.device)
-    mean = _alloc((samples, num_groups), torch.float32, input.device)
-    rstd = _alloc((samples, num_groups), torch.float32, input.device)
-    d_y, p_y = _desc_of(handle, "out", out)
-    d_m = _array_desc(DTYPE_FLOAT, (samples, num_groups))
+        out = _new(input, input.shape, input.dtype)
+    mean, rstd = _new(input, stats, torch.float32), _new(input, stats, torch.float32)
+    p_y = _address(handle, "out", out)
+    specs = lambda: [_spec(t) for t in (input, weight, bias, sample_ends, out)] + [(torch.float32, stats)]  # noqa: E731
+    plan = _call_plan(handle, ("norm", num_groups, input.shape, input.dtype, out.shape, out.dtype, _spec(weight),
+                               _spec(bias), _spec(sample_ends)), specs,
+                      lambda plan, size: check("mluOpGetGroupNormActForwardWorkspaceSize",
+                                               lib().mluOpGetGroupNormActForwardWorkspaceSize(
+                                                   handle.ptr, plan.d[0], plan.d[3], num_groups, ctypes.byref(size))))
+    d_x, d_w, d_b, d_e, d_y, d_m = plan.d
+    workspace = _workspace(input, plan.workspace)
     check("mluOpGroupNormActForward",
-          lib().mluOpGroupNormActForward(handle.ptr, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, num_groups, epsilon,
-                                         GROUP_NORM_ACTS[activation], _ptr(workspace), size, d_y, p_y, d_m, _ptr(mean),
-                                         d_m, _ptr(rstd)))
+          lib().mluOpGroupNormActForward(handle.ptr, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, num_groups, epsilon, act,
+                                         workspace.data_ptr(), plan.workspace, d_y, p_y, d_m, mean.data_ptr(), d_m,
+                                         rstd.data_ptr()))
     return out, mean, rstd
 
 
@@ -824,31 +862,34 @@ def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd
     tensor, may be output_grad.
     """
     import torch
-    if activation not in GROUP_NORM_ACTS:
-        raise ValueError("activation is one of %s" % ", ".join(GROUP_NORM_ACTS))
-    d_g, p_g = _desc_of(handle, "output_grad", output_grad)
-    d_x, p_x = _desc_of(handle, "input", input)
-    d_w, p_w = _desc_of(handle, "weight", weight)
-    d_b, p_b = _desc_of(handle, "bias", bias)
-    d_e, p_e = _desc_of(handle, "sample_ends", sample_ends)
-    d_m, p_m = _desc_of(handle, "mean", mean)
-    d_r, p_r = _desc_of(handle, "rstd", rstd)
+    act = _activation(activation)
+    p_g = _address(handle, "output_grad", output_grad)
+    p_x = _address(handle, "input", input)
+    p_w = None if weight is None else _address(handle, "weight", weight)
+    p_b = None if bias is None else _address(handle, "bias", bias)
+    p_e = None if sample_ends is None else _address(handle, "sample_ends", sample_ends)
+    p_m, p_r = _address(handle, "mean", mean), _address(handle, "rstd", rstd)
     num_groups = int(num_groups)
-    workspace, size = _group_norm_workspace(handle, "mluOpGetGroupNormActBackwardWorkspaceSize", d_x, d_e, num_groups,
-                                            input.device)
     if out is None:
-        out = _alloc(input.shape, input.dtype, input.device)
-    d_o, p_o = _desc_of(handle, "out", out)
-    weight_grad = bias_grad = None
+        out = _new(input, input.shape, input.dtype)
+    p_o = _address(handle, "out", out)
+    weight_grad = bias_grad = p_wg = p_bg = None
     if affine_grad:
-        weight_grad = _alloc((input.shape[-1],), affine_grad_dtype or torch.float32, input.device)
-        bias_grad = _alloc((input.shape[-1],), affine_grad_dtype or torch.float32, input.device)
-    d_wg, p_wg = _desc_of(handle, "weight_grad", weight_grad)
-    d_bg, p_bg = _desc_of(handle, "bias_grad", bias_grad)
+        weight_grad = _new(input, input.shape[-1:], affine_grad_dtype or torch.float32)
+        bias_grad = _new(input, input.shape[-1:], affine_grad_dtype or torch.float32)
+        p_wg, p_bg = weight_grad.data_ptr(), bias_grad.data_ptr()
+    tensors = (output_grad, input, weight, bias, sample_ends, mean, rstd, out, weight_grad, bias_grad)
+    plan = _call_plan(handle, ("norm_grad", num_groups) + tuple([_spec(t) for t in tensors]),
+                      lambda: [_spec(t) for t in tensors],
+                      lambda plan, size: check("mluOpGetGroupNormActBackwardWorkspaceSize",
+                                               lib().mluOpGetGroupNormActBackwardWorkspaceSize(
+                                                   handle.ptr, plan.d[1], plan.d[4], num_groups, ctypes.byref(size))))
+    d_g, d_x, d_w, d_b, d_e, d_m, d_r, d_o, d_wg, d_bg = plan.d
+    workspace = _workspace(input, plan.workspace)
     check("mluOpGroupNormActBackward",
           lib().mluOpGroupNormActBackward(handle.ptr, d_g, p_g, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, d_m, p_m, d_r,
-                                          p_r, num_groups, GROUP_NORM_ACTS[activation], _ptr(workspace), size, d_o,
-                                          p_o, d_wg, p_wg, d_bg, p_bg))
+                                          p_r, num_groups, act, workspace.data_ptr(), plan.workspace, d_o, p_o, d_wg,
+                                          p_wg, d_bg, p_bg))
     return out, weight_grad, bias_grad
 
 
@@ -924,7 +965,7 @@ class MultiTensorAdamW:
             raise ValueError("the tensors lie on device %s, the handle on CUDA device %d" % (self.device, handle.device))
         dtype = grads[0].dtype
         for g, n in zip(grads, self.numels):
-            if g.dtype is not dtype or g.numel() != n or g.get_device() != self.device or not g.is_contiguous():
+            if g.numel() != n or g.dtype is not dtype or g.get_device() != self.device or not g.is_contiguous():
                 raise ValueError("gradients are dense, of one type, on the parameters' device and of their sizes")
         for name, t, n in (("grad_scale", grad_scale, 1), ("schedule", schedule, 3)):
             if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.get_device() != self.device
@@ -946,12 +987,15 @@ def grouped_matmul_forward(handle, input, weight, group_ends, out=None):
     [G] on the device: group g's rows end there, the next group's begin.  Rows behind the last
     group's end: zeros.
     """
-    d_x, p_x = _desc_of(handle, "input", input)
-    d_w, p_w = _desc_of(handle, "weight", weight)
-    d_e, p_e = _desc_of(handle, "group_ends", group_ends)
+    p_x, p_w, p_e = (_address(handle, "input", input), _address(handle, "weight", weight),
+                     _address(handle, "group_ends", group_ends))
     if out is None:
-        out = _alloc((input.shape[0], weight.shape[-1]), input.dtype, input.device)
-    d_y, p_y = _desc_of(handle, "out", out)
+        out = _new(input, (input.shape[0], weight.shape[-1]), input.dtype)
+    p_y = _address(handle, "out", out)
+    tensors = (input, weight, group_ends, out)
+    plan = _call_plan(handle, ("product", input.shape, input.dtype, weight.shape, weight.dtype, group_ends.shape,
+                               group_ends.dtype, out.shape, out.dtype), lambda: [_spec(t) for t in tensors])
+    d_x, d_w, d_e, d_y = plan.d
     check("mluOpGroupedMatMulForward",
           lib().mluOpGroupedMatMulForward(handle.ptr, d_x, p_x, d_w, p_w, d_e, p_e, d_y, p_y))
     return out
@@ -960,33 +1004,39 @@ def grouped_matmul_forward(handle, input, weight, group_ends, out=None):
 def grouped_matmul_backward_input(handle, output_grad, weight, group_ends, out=None):
     """input_grad [rows,Ci] with input_grad[r] = output_grad[r] @ weight[g].T through
     mluOpGroupedMatMulBackwardInput (the forward call's arguments)."""
-    d_g, p_g = _desc_of(handle, "output_grad", output_grad)
-    d_w, p_w = _desc_of(handle, "weight", weight)
-    d_e, p_e = _desc_of(handle, "group_ends", group_ends)
+    p_g, p_w, p_e = (_address(handle, "output_grad", output_grad), _address(handle, "weight", weight),
+                     _address(handle, "group_ends", group_ends))
     if out is None:
-        out = _alloc((output_grad.shape[0], weight.shape[-2]), output_grad.dtype, output_grad.device)
-    d_x, p_x = _desc_of(handle, "out", out)
+        out = _new(output_grad, (output_grad.shape[0], weight.shape[-2]), output_grad.dtype)
+    p_x = _address(handle, "out", out)
+    tensors = (output_grad, weight, group_ends, out)
+    plan = _call_plan(handle, ("product", output_grad.shape, output_grad.dtype, weight.shape, weight.dtype,
+                               group_ends.shape, group_ends.dtype, out.shape, out.dtype),
+                      lambda: [_spec(t) for t in tensors])
+    d_g, d_w, d_e, d_x = plan.d
     check("mluOpGroupedMatMulBackwardInput",
           lib().mluOpGroupedMatMulBackwardInput(handle.ptr, d_g, p_g, d_w, p_w, d_e, p_e, d_x, p_x))
     return out
 
 
-def grouped_matmul_backward_weight(handle, input, output_grad, group_ends, dtype=None, workspace=None, out=None):
+def grouped_matmul_backward_weight(handle, input, output_grad, group_ends, dtype=None, out=None):
     """weight_grad [G,Ci,Co] with weight_grad[g] = input[rows of g].T @ output_grad[rows of g] through
     mluOpGroupedMatMulBackwardWeight; dtype: input's (default) or float32."""
-    import torch
-    d_x, p_x = _desc_of(handle, "input", input)
-    d_g, p_g = _desc_of(handle, "output_grad", output_grad)
-    d_e, p_e = _desc_of(handle, "group_ends", group_ends)
+    p_x, p_g, p_e = (_address(handle, "input", input), _address(handle, "output_grad", output_grad),
+                     _address(handle, "group_ends", group_ends))
     if out is None:
-        out = _alloc((group_ends.shape[0], input.shape[-1], output_grad.shape[-1]), dtype or input.dtype, input.device)
-    d_w, p_w = _desc_of(handle, "out", out)
-    size = _szt(0)
-    check("mluOpGetGroupedMatMulBackwardWeightWorkspaceSize",
-          lib().mluOpGetGroupedMatMulBackwardWeightWorkspaceSize(handle.ptr, d_x, d_g, d_w, ctypes.byref(size)))
-    if workspace is None or workspace.numel() < size.value:
-        workspace = _alloc((size.value,), torch.uint8, input.device)
+        out = _new(input, (group_ends.shape[0], input.shape[-1], output_grad.shape[-1]), dtype or input.dtype)
+    p_w = _address(handle, "out", out)
+    tensors = (input, output_grad, group_ends, out)
+    plan = _call_plan(handle, ("product_weight", input.shape, input.dtype, output_grad.shape, output_grad.dtype,
+                               group_ends.shape, group_ends.dtype, out.shape, out.dtype),
+                      lambda: [_spec(t) for t in tensors],
+                      lambda plan, size: check("mluOpGetGroupedMatMulBackwardWeightWorkspaceSize",
+                                               lib().mluOpGetGroupedMatMulBackwardWeightWorkspaceSize(
+                                                   handle.ptr, plan.d[0], plan.d[1], plan.d[3], ctypes.byref(size))))
+    d_x, d_g, d_e, d_w = plan.d
+    workspace = _workspace(input, plan.workspace)
     check("mluOpGroupedMatMulBackwardWeight",
-          lib().mluOpGroupedMatMulBackwardWeight(handle.ptr, d_x, p_x, d_g, p_g, d_e, p_e, _ptr(workspace), size.value,
-                                                 d_w, p_w))
+          lib().mluOpGroupedMatMulBackwardWeight(handle.ptr, d_x, p_x, d_g, p_g, d_e, p_e, workspace.data_ptr(),
+                                                 plan.workspace, d_w, p_w))
     return out

@@ -25,8 +25,32 @@ bool takeStickyDeviceError(mluOpHandle_t handle, const char *api) {
   *word = 0;
   LOG(ERROR) << api << " an earlier asynchronous call on this handle reported device error bits " << bits
              << " (1: hash table full, 4: look-back wait gave up, 0x100 and up: a bounded wait of a "
-             << "tensor-core kernel gave up); its outputs are not valid.";
+             << "kernel gave up); its outputs are not valid.";
   return true;
+}
+
+int32_t *stickyDeviceWord(mluOpHandle_t handle) {
+  void *word = nullptr;
+  if (cudaHostGetDevicePointer(&word, handle->host_words + mluOpContext::kStickyWord, 0) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return nullptr;
+  }
+  return static_cast<int32_t *>(word);
+}
+
+mluOpStatus_t reportIfRequested(mluOpHandle_t handle, const char *api) {
+  if (!checkStatusRequested()) return MLUOP_STATUS_SUCCESS;
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(handle->queue, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) {
+    (void)cudaGetLastError();
+    return MLUOP_STATUS_SUCCESS;
+  }
+  const cudaError_t err = cudaStreamSynchronize(handle->queue);
+  if (err != cudaSuccess) {
+    LOG(ERROR) << api << " execution failed: " << cudaGetErrorString(err);
+    return MLUOP_STATUS_EXECUTION_FAILED;
+  }
+  return takeStickyDeviceError(handle, api) ? MLUOP_STATUS_EXECUTION_FAILED : MLUOP_STATUS_SUCCESS;
 }
 
 DeviceGuard::DeviceGuard(mluOpHandle_t handle) {

@@ -63,6 +63,13 @@ bool checkStatusRequested();
 // synchronisation: only errors that have already reached the host are seen.
 bool takeStickyDeviceError(mluOpHandle_t handle, const char *api);
 
+// Where kernels of this handle record such an error: the sticky word's device address (null if it has none).
+int32_t *stickyDeviceWord(mluOpHandle_t handle);
+
+// The end of an asynchronous entry point: with checkStatusRequested(), and outside of a stream capture, waits for the
+// handle's queue and reports an error that its work recorded.
+mluOpStatus_t reportIfRequested(mluOpHandle_t handle, const char *api);
+
 // Makes the handle's device the current one for the guard's lifetime, so that a call works whichever
 // device the calling thread has selected.
 class DeviceGuard {

@@ -17,6 +17,11 @@
 // sums for sample s go to slot block + s, which is unique and makes the slots of one
 // sample neighbours, whatever the samples' sizes (they are known on the device only).
 //
+// Few rows: the three launches would take longer than their work.  There one block takes a
+// slice of channels that holds whole groups (forward: of one sample; backward: of all
+// samples one after the other, so that the affine gradients stay in the block) and does
+// all three steps; the second reading comes from L1 or L2.
+//
 // Variance: pass 1 sums x - k and (x - k)^2 with k the block's first value of that
 // channel, which is within a few deviations of the mean; the blocks' (mean, sum of
 // squared deviations) pairs are joined without cancellation.
@@ -25,10 +30,11 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <numeric>
 
-#include "core/convert.cuh"
 #include "core/trace.h"
 #include "core/type.h"
+#include "kernels/group_norm_act/group_norm_act_device.cuh"
 
 namespace mluop {
 namespace group_norm_act {
@@ -37,337 +43,303 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;  // rows a thread has in flight
+constexpr int kSmallThreads = 512;
+constexpr int kSmallTurns = 16;  // rows a thread of the one-launch form takes, at most
 
-struct Rows {
-  int64_t rows, samples, sample_rows, block_rows;
-  const int32_t *ends;  // null: samples of sample_rows rows
+// A block's threads: `columns` side by side on a row, `row_threads` rows at a time.
+struct Lanes {
+  int columns, row_threads;
 };
 
-// First row of sample s (s <= samples); within [0, rows] whatever the entries hold.
-__device__ __forceinline__ int64_t sampleStart(const Rows &r, int64_t s) {
-  if (s <= 0) return 0;
-  if (!r.ends) return s * r.sample_rows;
-  const int64_t e = r.ends[s - 1];
-  return e < 0 ? 0 : (e > r.rows ? r.rows : e);
-}
-
-// The sample that row `row` belongs to (`samples` behind the last one); called by the whole block.
-__device__ __forceinline__ int64_t sampleOf(const Rows &r, int64_t row) {
-  if (!r.ends) return r.sample_rows ? row / r.sample_rows : r.samples;
-  int64_t before = 0;
-  for (int64_t base = 0; base < r.samples; base += kThreads) {
-    const int64_t i = base + threadIdx.x;
-    before += __syncthreads_count(i < r.samples && r.ends[i] <= row);
-  }
-  return before;
-}
-
-__device__ __forceinline__ float loadAffine(const void *p, bool is_float, const float *, int c) {
-  return static_cast<const float *>(p)[c];
-}
-template <typename T>
-__device__ __forceinline__ float loadAffine(const void *p, bool is_float, const T *, int c) {
-  return is_float ? static_cast<const float *>(p)[c] : toFloat(static_cast<const T *>(p)[c]);
-}
-
-template <int ACT>
-__device__ __forceinline__ float activate(float u) {
-  if (ACT == MLUOP_GROUP_NORM_ACT_RELU) return u < 0.0f ? 0.0f : u;  // (NaN stays)
-  if (ACT == MLUOP_GROUP_NORM_ACT_SILU) return __fdividef(u, 1.0f + __expf(-u));
-  return u;
-}
-// dy * act'(u)
-template <int ACT>
-__device__ __forceinline__ float activateGrad(float dy, float u) {
-  if (ACT == MLUOP_GROUP_NORM_ACT_RELU) return u > 0.0f ? dy : 0.0f;
-  if (ACT == MLUOP_GROUP_NORM_ACT_SILU) {
-    const float s = __fdividef(1.0f, 1.0f + __expf(-u));
-    return dy * (s * (1.0f + u * (1.0f - s)));
-  }
-  return dy;
-}
-
-// Adds (a, b) of each channel over the block's row threads; the sums are returned to row thread 0.
-template <int VEC>
-__device__ __forceinline__ void addOverRowThreads(float (&a)[VEC], float (&b)[VEC], int column, int row, int columns,
-                                                  int row_threads, bool active, float2 *scratch) {
+// A thread's sums (a, b) of each of its channels, added over the block's row threads in a fixed order; store(channel, sum)
+// is called once for each of the block's channels.  The values lie side by side in `scratch`, so that lanes read and
+// write neighbouring words, and are added in two steps, `parts` threads to a channel first.
+template <int VEC, int THREADS, typename F>
+__device__ __forceinline__ void joinRowThreads(const Two (&a)[(VEC + 1) / 2], const Two (&b)[(VEC + 1) / 2], Lanes l,
+                                               float2 *scratch, F store) {
+  const int tid = threadIdx.x, used = l.columns * l.row_threads;
   __syncthreads();
-  if (active) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) scratch[(row * VEC + j) * columns + column] = make_float2(a[j], b[j]);
-  }
-  for (int half = row_threads; half > 1;) {
-    const int next = (half + 1) / 2;
-    __syncthreads();
-    if (active && row + next < half) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float2 mine = scratch[(row * VEC + j) * columns + column];
-        const float2 other = scratch[((row + next) * VEC + j) * columns + column];
-        scratch[(row * VEC + j) * columns + column] = make_float2(mine.x + other.x, mine.y + other.y);
-      }
-    }
-    half = next;
-  }
-  if (active && row == 0) {
+  if (tid < used) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const float2 sum = scratch[j * columns + column];
-      a[j] = sum.x;
-      b[j] = sum.y;
+      const float2 x = split(a[j / 2]), y = split(b[j / 2]);
+      scratch[j * used + tid] = j % 2 ? make_float2(x.y, y.y) : make_float2(x.x, y.x);
     }
   }
-}
-
-// Per channel of the thread: what the normalisation needs.
-template <int VEC>
-struct Channel {
-  float mean[VEC], rstd[VEC], gamma[VEC], beta[VEC];
-};
-template <typename T, int VEC>
-__device__ __forceinline__ void loadChannels(Channel<VEC> &c, const float *mean, const float *rstd, const void *weight,
-                                             const void *bias, bool float_affine, int64_t sample, int first, int groups,
-                                             int group_channels) {
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    const int64_t q = sample * groups + (first + j) / group_channels;
-    c.mean[j] = mean[q];
-    c.rstd[j] = rstd[q];
-    c.gamma[j] = weight ? loadAffine(weight, float_affine, (const T *)nullptr, first + j) : 1.0f;
-    c.beta[j] = bias ? loadAffine(bias, float_affine, (const T *)nullptr, first + j) : 0.0f;
-  }
-}
-// The activation's argument, rounded after every operation: a value next to the border of relu falls on the same
-// side in the forward pass, in both backward passes and in the formula evaluated step by step.
-template <int VEC>
-__device__ __forceinline__ float normalised(const Channel<VEC> &c, int j, float x) {
-  return __fmul_rn(__fsub_rn(x, c.mean[j]), c.rstd[j]);
-}
-template <int VEC>
-__device__ __forceinline__ float affine(const Channel<VEC> &c, int j, float xhat) {
-  return __fadd_rn(__fmul_rn(xhat, c.gamma[j]), c.beta[j]);
-}
-
-// Pass 1 forward: partial[slot][channel] = (mean, sum of squared deviations) of the block's rows of a sample.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads)
-statisticsKernel(const T *x, Rows r, int channels, int columns, int row_threads, float2 *partial) {
-  extern __shared__ float2 scratch[];
-  const int column = threadIdx.x % columns, row = threadIdx.x / columns;
-  const int first = (blockIdx.y * columns + column) * VEC;
-  const bool active = row < row_threads && first < channels;
-  const int64_t begin = (int64_t)blockIdx.x * r.block_rows;
-  const int64_t end = begin + r.block_rows < r.rows ? begin + r.block_rows : r.rows;
-  int64_t sample = sampleOf(r, begin);
-  for (int64_t at = begin; at < end && sample < r.samples; ++sample) {
-    int64_t stop = sampleStart(r, sample + 1);
-    stop = stop < end ? stop : end;
-    if (stop <= at) continue;
-    float k[VEC], s[VEC], q[VEC];
-    if (active) {
-      const Pack<VEC, T> p = loadPack<VEC>(x + at * channels + first);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) k[j] = toFloat(p.v[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) s[j] = q[j] = 0.0f;
-    if (active) {
-      int64_t i = at + row;
-      for (; i + (kUnroll - 1) * row_threads < stop; i += kUnroll * row_threads) {
-        Pack<VEC, T> p[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) p[u] = loadPack<VEC>(x + (i + u * row_threads) * channels + first);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float d = toFloat(p[u].v[j]) - k[j];
-            s[j] += d;
-            q[j] += d * d;
-          }
-        }
-      }
-      for (; i < stop; i += row_threads) {
-        const Pack<VEC, T> p = loadPack<VEC>(x + i * channels + first);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float d = toFloat(p.v[j]) - k[j];
-          s[j] += d;
-          q[j] += d * d;
-        }
-      }
-    }
-    addOverRowThreads<VEC>(s, q, column, row, columns, row_threads, active, scratch);
-    if (active && row == 0) {
-      const float n = (float)(stop - at);
-      float2 *out = partial + (blockIdx.x + sample) * channels + first;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float off = s[j] / n;
-        const float squares = q[j] - s[j] * off;
-        out[j] = make_float2(k[j] + off, squares < 0.0f ? 0.0f : squares);  // (NaN stays)
-      }
-    }
-    at = stop;
-  }
-}
-
-// Sum over the block in a fixed order, returned to every thread.
-__device__ __forceinline__ double blockSum(double v, double *scratch) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0;
-  for (int w = 0; w < kThreads / 32; ++w) v += scratch[w];
-  return v;
-}
-
-// Pass 2 forward: one block per (sample, group).
-__global__ void __launch_bounds__(kThreads)
-joinStatisticsKernel(const float2 *partial, Rows r, int channels, int groups, float epsilon, float *mean, float *rstd) {
-  __shared__ double scratch[kThreads / 32];
-  const int64_t sample = blockIdx.x / groups;
-  const int group = blockIdx.x % groups, group_channels = channels / groups;
-  const int64_t begin = sampleStart(r, sample), end = sampleStart(r, sample + 1);
-  double m = 0.0, sq = 0.0;
-  if (end > begin) {
-    const int64_t b0 = begin / r.block_rows, b1 = (end - 1) / r.block_rows;
-    const int64_t items = (b1 - b0 + 1) * group_channels;
-    const double total = (double)(end - begin) * group_channels;
-    for (int64_t i = threadIdx.x; i < items; i += kThreads) {
-      const int64_t b = b0 + i / group_channels;
-      const int64_t from = b * r.block_rows > begin ? b * r.block_rows : begin;
-      const int64_t to = (b + 1) * r.block_rows < end ? (b + 1) * r.block_rows : end;
-      m += (double)(to - from) * partial[(b + sample) * channels + group * group_channels + i % group_channels].x;
+  const int items = VEC * l.columns;  // (j, column), column fastest
+  int parts = THREADS / items;
+  parts = parts < 1 ? 1 : (parts > l.row_threads ? l.row_threads : parts);
+  int rows = l.row_threads;
+  if (parts > 1) {
+    float2 s = make_float2(0.0f, 0.0f);
+    const int column = tid % l.columns, part = tid / l.columns % parts, j = tid / (l.columns * parts);
+    if (j < VEC) {
+      for (int row = part; row < l.row_threads; row += parts) {
+        const float2 v = scratch[j * used + row * l.columns + column];
+        s.x += v.x;
+        s.y += v.y;
+      }
     }
-    m = blockSum(m, scratch) / total;
-    for (int64_t i = threadIdx.x; i < items; i += kThreads) {
-      const int64_t b = b0 + i / group_channels;
-      const int64_t from = b * r.block_rows > begin ? b * r.block_rows : begin;
-      const int64_t to = (b + 1) * r.block_rows < end ? (b + 1) * r.block_rows : end;
-      const float2 v = partial[(b + sample) * channels + group * group_channels + i % group_channels];
-      const double d = (double)v.x - m;
-      sq += (double)v.y + (double)(to - from) * d * d;
-    }
-    sq = blockSum(sq, scratch) / total;
+    __syncthreads();
+    if (j < VEC) scratch[tid] = s;
+    __syncthreads();
+    rows = parts;
   }
-  if (threadIdx.x == 0) {
-    mean[blockIdx.x] = (float)m;
-    rstd[blockIdx.x] = (float)(1.0 / sqrt(sq + (double)epsilon));
+  for (int item = tid; item < items; item += THREADS) {
+    const int column = item % l.columns, j = item / l.columns;
+    float2 s = make_float2(0.0f, 0.0f);
+    for (int row = 0; row < rows; ++row) {
+      const float2 v = scratch[(j * rows + row) * l.columns + column];
+      s.x += v.x;
+      s.y += v.y;
+    }
+    store(column * VEC + j, s);
   }
 }
 
-// Pass 3 forward.
-template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(kThreads)
-normaliseKernel(const T *x, const void *weight, const void *bias, bool float_affine, const float *mean,
-                const float *rstd, Rows r, int channels, int groups, int columns, int row_threads, T *y) {
-  const int column = threadIdx.x % columns, row = threadIdx.x / columns;
-  const int first = (blockIdx.y * columns + column) * VEC;
-  const bool active = row < row_threads && first < channels;
-  const int64_t begin = (int64_t)(gridDim.x - 1 - blockIdx.x) * r.block_rows;
-  const int64_t end = begin + r.block_rows < r.rows ? begin + r.block_rows : r.rows;
-  int64_t sample = sampleOf(r, begin);
-  if (!active) return;
+// Calls body(first row, last row + 1, sample) for the parts of rows begin .. end-1 that belong to one sample each, and
+// rest(first row) for the rows of no sample; by the whole block.
+template <typename F, typename G>
+__device__ __forceinline__ void forSamples(const Rows &r, int64_t begin, int64_t end, F body, G rest) {
+  int64_t sample = samplesUpTo(r, begin);
   for (int64_t at = begin; at < end; ++sample) {
-    if (sample >= r.samples) {  // rows of no sample
-      Pack<VEC, T> zero;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) zero.v[j] = fromFloat<T>(0.0f);
-      for (int64_t i = at + row; i < end; i += row_threads) storePack<VEC>(y + i * channels + first, zero);
+    if (sample >= r.samples) {
+      rest(at);
       return;
     }
     int64_t stop = sampleStart(r, sample + 1);
     stop = stop < end ? stop : end;
     if (stop <= at) continue;
-    Channel<VEC> c;
-    loadChannels<T, VEC>(c, mean, rstd, weight, bias, float_affine, sample, first, groups, channels / groups);
-    int64_t i = at + row;
-    for (; i + (kUnroll - 1) * row_threads < stop; i += kUnroll * row_threads) {
-      Pack<VEC, T> p[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = loadPack<VEC>(x + (i + u * row_threads) * channels + first);
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          p[u].v[j] = fromFloat<T>(activate<ACT>(affine(c, j, normalised(c, j, toFloat(p[u].v[j])))));
-        storePack<VEC>(y + (i + u * row_threads) * channels + first, p[u]);
-      }
-    }
-    for (; i < stop; i += row_threads) {
-      Pack<VEC, T> p = loadPack<VEC>(x + i * channels + first);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        p.v[j] = fromFloat<T>(activate<ACT>(affine(c, j, normalised(c, j, toFloat(p.v[j])))));
-      storePack<VEC>(y + i * channels + first, p);
-    }
+    body(at, stop, sample);
     at = stop;
   }
 }
 
-// Pass 1 backward: partial[slot][channel] = (sum du, sum du xhat) of the block's rows of a sample.
-template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(kThreads)
-gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bool float_affine, const float *mean,
-               const float *rstd, Rows r, int channels, int groups, int columns, int row_threads, float2 *partial) {
+// Pass 1 forward: partial[slot][channel] = (mean, sum of squared deviations) of the block's rows of a sample.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads, 4)
+statisticsKernel(const T *x, Rows r, int channels, Lanes l, float2 *partial) {
   extern __shared__ float2 scratch[];
-  const int column = threadIdx.x % columns, row = threadIdx.x / columns;
-  const int first = (blockIdx.y * columns + column) * VEC;
-  const bool active = row < row_threads && first < channels;
+  constexpr int kPairs = (VEC + 1) / 2;
+  const int column = threadIdx.x % l.columns, row = threadIdx.x / l.columns;
+  const int first0 = blockIdx.y * l.columns * VEC, first = first0 + column * VEC;
+  const bool active = row < l.row_threads && first < channels;
   const int64_t begin = (int64_t)blockIdx.x * r.block_rows;
   const int64_t end = begin + r.block_rows < r.rows ? begin + r.block_rows : r.rows;
-  int64_t sample = sampleOf(r, begin);
-  for (int64_t at = begin; at < end && sample < r.samples; ++sample) {
-    int64_t stop = sampleStart(r, sample + 1);
-    stop = stop < end ? stop : end;
-    if (stop <= at) continue;
-    float a[VEC], b[VEC];
+  const int64_t step = (int64_t)l.row_threads * channels;
+  forSamples(r, begin, end, [&](int64_t at, int64_t stop, int64_t sample) {
+    Two a[kPairs], b[kPairs], minus_k[kPairs];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) a[j] = b[j] = 0.0f;
+    for (int j = 0; j < kPairs; ++j) a[j] = b[j] = minus_k[j] = two(0.0f, 0.0f);
     if (active) {
-      Channel<VEC> c;
-      loadChannels<T, VEC>(c, mean, rstd, weight, bias, float_affine, sample, first, groups, channels / groups);
-      int64_t i = at + row;
-      for (; i + (kUnroll - 1) * row_threads < stop; i += kUnroll * row_threads) {
-        Pack<VEC, T> p[kUnroll], g[kUnroll];
+      Values<T, VEC> k;
+      k.load(x + at * channels + first);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          p[u] = loadPack<VEC>(x + (i + u * row_threads) * channels + first);
-          g[u] = loadPack<VEC>(dy + (i + u * row_threads) * channels + first);
+      for (int j = 0; j < kPairs; ++j) minus_k[j] = k.pair(j) * two(-1.0f, -1.0f);
+      auto add = [&](const Values<T, VEC> &v) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const Two d = v.pair(j) + minus_k[j];
+          a[j] = a[j] + d;
+          b[j] = fma(d, d, b[j]);
         }
+      };
+      int left = (int)(stop - at) - row;  // rows from the thread's next one on
+      const T *from = x + (at + row) * channels + first;
+      for (; left > (kUnroll - 1) * l.row_threads; left -= kUnroll * l.row_threads, from += kUnroll * step) {
+        Values<T, VEC> v[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < kUnroll; ++u) v[u].load(from + u * step);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float xhat = normalised(c, j, toFloat(p[u].v[j]));
-            const float du = activateGrad<ACT>(toFloat(g[u].v[j]), affine(c, j, xhat));
-            a[j] += du;
-            b[j] += du * xhat;
-          }
-        }
+        for (int u = 0; u < kUnroll; ++u) add(v[u]);
       }
-      for (; i < stop; i += row_threads) {
-        const Pack<VEC, T> p = loadPack<VEC>(x + i * channels + first);
-        const Pack<VEC, T> g = loadPack<VEC>(dy + i * channels + first);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float xhat = normalised(c, j, toFloat(p.v[j]));
-          const float du = activateGrad<ACT>(toFloat(g.v[j]), affine(c, j, xhat));
-          a[j] += du;
-          b[j] += du * xhat;
-        }
+      for (; left > 0; left -= l.row_threads, from += step) {
+        Values<T, VEC> v;
+        v.load(from);
+        add(v);
       }
     }
-    addOverRowThreads<VEC>(a, b, column, row, columns, row_threads, active, scratch);
-    if (active && row == 0) {
-      float2 *out = partial + (blockIdx.x + sample) * channels + first;
+    const float n = (float)(stop - at);
+    float2 *out = partial + (blockIdx.x + sample) * channels + first0;
+    joinRowThreads<VEC, kThreads>(a, b, l, scratch, [&](int c, float2 s) {
+      if (first0 + c >= channels) return;
+      const float k = toFloat(x[at * channels + first0 + c]);
+      const float off = s.x / n, squares = s.y - s.x * off;
+      out[c] = make_float2(k + off, squares < 0.0f ? 0.0f : squares);  // (NaN stays)
+    });
+  }, [](int64_t) {});
+}
+
+// Sums over the block in a fixed order, returned to every thread.
+__device__ __forceinline__ double2 blockSum(double a, double b, double2 *scratch) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) out[j] = make_float2(a[j], b[j]);
-    }
-    at = stop;
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
   }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_double2(a, b);
+  __syncthreads();
+  a = b = 0.0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    a += scratch[w].x;
+    b += scratch[w].y;
+  }
+  return make_double2(a, b);
+}
+
+// The slots of a sample: those of blocks first .. last.
+struct SampleSlots {
+  int64_t begin, end;
+  int first, last;
+  __device__ __forceinline__ SampleSlots(const Rows &r, int64_t sample) {
+    begin = sampleStart(r, sample);
+    end = sampleStart(r, sample + 1);
+    const unsigned rows = (unsigned)r.block_rows;  // (fewer than 2^31 rows)
+    first = (int)((unsigned)begin / rows);
+    last = end > begin ? (int)((unsigned)(end - 1) / rows) : first - 1;
+  }
+};
+
+// Pass 2 forward: one block per (sample, group).  The blocks' means are joined as distances from the first one.
+__global__ void __launch_bounds__(kThreads)
+joinStatisticsKernel(const float2 *partial, Rows r, int channels, int groups, float epsilon, float *mean, float *rstd) {
+  __shared__ double2 scratch[kThreads / 32];
+  const int64_t sample = blockIdx.x / groups;
+  const int group = blockIdx.x % groups, group_channels = channels / groups;
+  const SampleSlots s(r, sample);
+  const int width = group_channels < kThreads ? group_channels : kThreads, depth = kThreads / width;
+  const int c0 = threadIdx.x % width, d = threadIdx.x / width;
+  double a = 0.0, b = 0.0, ref = 0.0;
+  if (s.last >= s.first && d < depth) {
+    const float2 *from = partial + sample * channels + (int64_t)group * group_channels;
+    ref = from[(int64_t)s.first * channels].x;
+    for (int c = c0; c < group_channels; c += width) {
+      for (int64_t k = s.first + d; k <= s.last; k += depth) {
+        const int64_t lo = k * r.block_rows > s.begin ? k * r.block_rows : s.begin;
+        const int64_t hi = (k + 1) * r.block_rows < s.end ? (k + 1) * r.block_rows : s.end;
+        const float2 v = from[k * channels + c];
+        const double n = (double)(hi - lo), off = (double)v.x - ref;
+        a += n * off;
+        b += (double)v.y + n * off * off;
+      }
+    }
+  }
+  const double2 sum = blockSum(a, b, scratch);
+  if (threadIdx.x == 0) {
+    float m = 0.0f;
+    double var = 0.0;
+    if (s.last >= s.first) {
+      const double n = (double)(s.end - s.begin) * group_channels, off = sum.x / n;
+      m = (float)(ref + off);
+      var = sum.y / n - off * off;
+      var = var < 0.0 ? 0.0 : var;  // (NaN stays)
+    }
+    mean[blockIdx.x] = m;
+    rstd[blockIdx.x] = (float)(1.0 / sqrt(var + (double)epsilon));
+  }
+}
+
+// Pass 3 forward.
+template <typename T, int VEC, int ACT, bool UNIFORM>
+__global__ void __launch_bounds__(kThreads, 4)
+normaliseKernel(const T *x, const void *weight, const void *bias, bool float_affine, const float *mean,
+                const float *rstd, Rows r, int channels, int groups, Lanes l, T *y) {
+  constexpr int kPairs = (VEC + 1) / 2;
+  const int column = threadIdx.x % l.columns, row = threadIdx.x / l.columns;
+  const int first = (blockIdx.y * l.columns + column) * VEC;
+  const bool active = row < l.row_threads && first < channels;
+  const int64_t begin = (int64_t)(gridDim.x - 1 - blockIdx.x) * r.block_rows;
+  const int64_t end = begin + r.block_rows < r.rows ? begin + r.block_rows : r.rows;
+  const int64_t step = (int64_t)l.row_threads * channels;
+  forSamples(r, begin, end, [&](int64_t at, int64_t stop, int64_t sample) {
+    if (!active) return;
+    Norm<VEC, UNIFORM> c;
+    loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, channels / groups);
+    auto put = [&](T *to, const Values<T, VEC> &v) {
+      Two o[kPairs];
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) o[j] = activate<ACT>(c.affine(j, c.xhat(j, v.pair(j))));
+      Values<T, VEC>::store(to, o);
+    };
+    int left = (int)(stop - at) - row;
+    const T *from = x + (at + row) * channels + first;
+    T *to = y + (at + row) * channels + first;
+    for (; left > (kUnroll - 1) * l.row_threads; left -= kUnroll * l.row_threads, from += kUnroll * step, to += kUnroll * step) {
+      Values<T, VEC> v[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) v[u].load(from + u * step);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) put(to + u * step, v[u]);
+    }
+    for (; left > 0; left -= l.row_threads, from += step, to += step) {
+      Values<T, VEC> v;
+      v.load(from);
+      put(to, v);
+    }
+  }, [&](int64_t at) {
+    if (!active) return;
+    for (int64_t i = at + row; i < end; i += l.row_threads) Values<T, VEC>::storeZero(y + i * channels + first);
+  });
+}
+
+// Pass 1 backward: partial[slot][channel] = (sum du, sum du xhat) of the block's rows of a sample.
+template <typename T, int VEC, int ACT, bool UNIFORM>
+__global__ void __launch_bounds__(kThreads, 3)
+gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bool float_affine, const float *mean,
+               const float *rstd, Rows r, int channels, int groups, Lanes l, float2 *partial) {
+  extern __shared__ float2 scratch[];
+  constexpr int kPairs = (VEC + 1) / 2;
+  const int column = threadIdx.x % l.columns, row = threadIdx.x / l.columns;
+  const int first0 = blockIdx.y * l.columns * VEC, first = first0 + column * VEC;
+  const bool active = row < l.row_threads && first < channels;
+  const int64_t begin = (int64_t)blockIdx.x * r.block_rows;
+  const int64_t end = begin + r.block_rows < r.rows ? begin + r.block_rows : r.rows;
+  const int64_t step = (int64_t)l.row_threads * channels;
+  forSamples(r, begin, end, [&](int64_t at, int64_t stop, int64_t sample) {
+    Two a[kPairs], b[kPairs];
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) a[j] = b[j] = two(0.0f, 0.0f);
+    if (active) {
+      Norm<VEC, UNIFORM> c;
+      loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, channels / groups);
+      auto add = [&](const Values<T, VEC> &v, const Values<T, VEC> &g) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const Two xh = c.xhat(j, v.pair(j));
+          const Two du = activateGrad<ACT>(g.pair(j), c.affine(j, xh));
+          a[j] = a[j] + du;
+          b[j] = fma(du, xh, b[j]);
+        }
+      };
+      int left = (int)(stop - at) - row;
+      const int64_t offset = (at + row) * channels + first;
+      const T *from = x + offset, *from_g = dy + offset;
+      constexpr int kRows = kUnroll / 2;
+      for (; left > (kRows - 1) * l.row_threads; left -= kRows * l.row_threads, from += kRows * step, from_g += kRows * step) {
+        Values<T, VEC> v[kRows], g[kRows];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+          v[u].load(from + u * step);
+          g[u].load(from_g + u * step);
+        }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) add(v[u], g[u]);
+      }
+      if (left > 0) {
+        Values<T, VEC> v, g;
+        v.load(from);
+        g.load(from_g);
+        add(v, g);
+      }
+    }
+    float2 *out = partial + (blockIdx.x + sample) * channels + first0;
+    joinRowThreads<VEC, kThreads>(a, b, l, scratch, [&](int c, float2 s) {
+      if (first0 + c < channels) out[c] = s;
+    });
+  }, [](int64_t) {});
 }
 
 // Pass 2 backward: one block per (sample, group): the sample's sums per channel, and the group's two means.
@@ -375,11 +347,10 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 joinGradSumsKernel(const float2 *partial, const void *weight, bool float_affine, Rows r, int channels, int groups,
                    float2 *sample_sums, float2 *group_means) {
-  __shared__ double scratch[kThreads / 32];
-  __shared__ double2 lanes[kThreads];
+  __shared__ double2 scratch[kThreads / 32], lanes[kThreads];
   const int64_t sample = blockIdx.x / groups;
   const int group = blockIdx.x % groups, group_channels = channels / groups;
-  const int64_t begin = sampleStart(r, sample), end = sampleStart(r, sample + 1);
+  const SampleSlots s(r, sample);
   // a tile of up to 32 channels side by side, the other threads along the slots
   const int width = group_channels < 32 ? group_channels : 32, depth = kThreads / width;
   const int c = threadIdx.x % width, d = threadIdx.x / width;
@@ -388,9 +359,9 @@ joinGradSumsKernel(const float2 *partial, const void *weight, bool float_affine,
     const int channel = group * group_channels + base + c;
     const bool active = d < depth && base + c < group_channels;
     double a = 0.0, b = 0.0;
-    if (active && end > begin) {
-      const int64_t last = (end - 1) / r.block_rows;
-      for (int64_t k = begin / r.block_rows + d; k <= last; k += depth) {
+    if (active) {
+#pragma unroll 4
+      for (int64_t k = s.first + d; k <= s.last; k += depth) {
         const float2 v = partial[(k + sample) * channels + channel];
         a += v.x;
         b += v.y;
@@ -405,40 +376,34 @@ joinGradSumsKernel(const float2 *partial, const void *weight, bool float_affine,
         b += lanes[i * width + c].y;
       }
       sample_sums[sample * channels + channel] = make_float2((float)a, (float)b);
-      const double gamma = weight ? (double)loadAffine(weight, float_affine, (const T *)nullptr, channel) : 1.0;
+      const double gamma = weight ? (double)loadAffine<T>(weight, float_affine, channel) : 1.0;
       m1 += gamma * a;
       m2 += gamma * b;
     }
   }
-  m1 = blockSum(m1, scratch);
-  m2 = blockSum(m2, scratch);
+  const double2 sum = blockSum(m1, m2, scratch);
   if (threadIdx.x == 0) {
-    const double n = end > begin ? (double)(end - begin) * group_channels : 1.0;
-    group_means[blockIdx.x] = make_float2((float)(m1 / n), (float)(m2 / n));
+    const double n = s.end > s.begin ? (double)(s.end - s.begin) * group_channels : 1.0;
+    group_means[blockIdx.x] = make_float2((float)(sum.x / n), (float)(sum.y / n));
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void storeAffineGrad(void *p, bool is_float, int c, double v) {
-  if (is_float) static_cast<float *>(p)[c] = (float)v;
-  else static_cast<T *>(p)[c] = fromFloat<T>((float)v);
-}
-
 // Pass 3 backward: the input gradient; the first blocks also add the samples' sums to the affine gradients.
-template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, int VEC, int ACT, bool UNIFORM>
+__global__ void __launch_bounds__(kThreads, 3)
 inputGradKernel(const T *dy, const T *x, const void *weight, const void *bias, bool float_affine, const float *mean,
                 const float *rstd, const float2 *sample_sums, const float2 *group_means, Rows r, int channels,
-                int groups, int columns, int row_threads, T *dx, void *weight_grad, void *bias_grad,
-                bool float_affine_grad) {
-  const int column = threadIdx.x % columns, row = threadIdx.x / columns;
-  const int first = (blockIdx.y * columns + column) * VEC;
-  const bool active = row < row_threads && first < channels;
+                int groups, Lanes l, T *dx, void *weight_grad, void *bias_grad, bool float_affine_grad) {
+  constexpr int kPairs = (VEC + 1) / 2;
+  const int column = threadIdx.x % l.columns, row = threadIdx.x / l.columns;
+  const int first = (blockIdx.y * l.columns + column) * VEC, group_channels = channels / groups;
+  const bool active = row < l.row_threads && first < channels;
   if (weight_grad) {
     const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     const int64_t all = (int64_t)gridDim.x * gridDim.y * kThreads;
     for (int64_t ch = block * kThreads + threadIdx.x; ch < channels; ch += all) {
       double a = 0.0, b = 0.0;
+#pragma unroll 4
       for (int64_t s = 0; s < r.samples; ++s) {
         const float2 v = sample_sums[s * channels + ch];
         a += v.x;
@@ -450,51 +415,205 @@ inputGradKernel(const T *dy, const T *x, const void *weight, const void *bias, b
   }
   const int64_t begin = (int64_t)(gridDim.x - 1 - blockIdx.x) * r.block_rows;
   const int64_t end = begin + r.block_rows < r.rows ? begin + r.block_rows : r.rows;
-  int64_t sample = sampleOf(r, begin);
-  if (!active) return;
-  const int group_channels = channels / groups;
-  for (int64_t at = begin; at < end; ++sample) {
-    if (sample >= r.samples) {  // rows of no sample
-      Pack<VEC, T> zero;
+  const int64_t step = (int64_t)l.row_threads * channels;
+  forSamples(r, begin, end, [&](int64_t at, int64_t stop, int64_t sample) {
+    if (!active) return;
+    Norm<VEC, UNIFORM> c;
+    loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, group_channels);
+    constexpr int kGroups = Norm<VEC, UNIFORM>::kGroups;
+    Two minus_m1[kGroups], minus_m2[kGroups];
+    const float2 *means = group_means + sample * groups;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) zero.v[j] = fromFloat<T>(0.0f);
-      for (int64_t i = at + row; i < end; i += row_threads) storePack<VEC>(dx + i * channels + first, zero);
-      return;
+    for (int j = 0; j < kGroups; ++j) {
+      minus_m1[j] = ofPair<UNIFORM ? 2 : VEC>(first, j, [&](int ch) { return -means[(UNIFORM ? first : ch) / group_channels].x; });
+      minus_m2[j] = ofPair<UNIFORM ? 2 : VEC>(first, j, [&](int ch) { return -means[(UNIFORM ? first : ch) / group_channels].y; });
     }
-    int64_t stop = sampleStart(r, sample + 1);
-    stop = stop < end ? stop : end;
-    if (stop <= at) continue;
-    Channel<VEC> c;
-    loadChannels<T, VEC>(c, mean, rstd, weight, bias, float_affine, sample, first, groups, group_channels);
-    float m1[VEC], m2[VEC];
+    auto put = [&](T *to, const Values<T, VEC> &v, const Values<T, VEC> &g) {
+      Two o[kPairs];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float2 v = group_means[sample * groups + (first + j) / group_channels];
-      m1[j] = v.x;
-      m2[j] = v.y;
-    }
-    for (int64_t i = at + row; i < stop; i += 2 * row_threads) {
-      const bool two = i + row_threads < stop;
-      Pack<VEC, T> p[2], g[2];
-      p[0] = loadPack<VEC>(x + i * channels + first);
-      g[0] = loadPack<VEC>(dy + i * channels + first);
-      if (two) {
-        p[1] = loadPack<VEC>(x + (i + row_threads) * channels + first);
-        g[1] = loadPack<VEC>(dy + (i + row_threads) * channels + first);
+      for (int j = 0; j < kPairs; ++j) {
+        const int q = UNIFORM ? 0 : j;
+        const Two xh = c.xhat(j, v.pair(j));
+        const Two du = activateGrad<ACT>(g.pair(j), c.affine(j, xh));
+        o[j] = fma(xh, minus_m2[q], fma(du, c.gamma[j], minus_m1[q])) * c.rstd[q];
+      }
+      Values<T, VEC>::store(to, o);
+    };
+    int left = (int)(stop - at) - row;
+    const int64_t offset = (at + row) * channels + first;
+    const T *from = x + offset, *from_g = dy + offset;
+    T *to = dx + offset;
+    constexpr int kRows = kUnroll / 2;
+    for (; left > (kRows - 1) * l.row_threads; left -= kRows * l.row_threads, from += kRows * step, from_g += kRows * step, to += kRows * step) {
+      Values<T, VEC> v[kRows], g[kRows];
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        v[u].load(from + u * step);
+        g[u].load(from_g + u * step);
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (u == 1 && !two) break;
+      for (int u = 0; u < kRows; ++u) put(to + u * step, v[u], g[u]);
+    }
+    if (left > 0) {
+      Values<T, VEC> v, g;
+      v.load(from);
+      g.load(from_g);
+      put(to, v, g);
+    }
+  }, [&](int64_t at) {
+    if (!active) return;
+    for (int64_t i = at + row; i < end; i += l.row_threads) Values<T, VEC>::storeZero(dx + i * channels + first);
+  });
+}
+
+// All three steps in one block: the slice of l.columns vectors from column blockIdx.x * l.columns on.
+template <typename T, int VEC, int ACT, bool UNIFORM, bool BACKWARD>
+__global__ void __launch_bounds__(kSmallThreads, 1)
+sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool float_affine, float *mean, float *rstd,
+            Rows r, int channels, int groups, Lanes l, float epsilon, T *out, void *weight_grad, void *bias_grad,
+            bool float_affine_grad) {
+  constexpr int kPairs = (VEC + 1) / 2, kGroups = UNIFORM ? 1 : kPairs;
+  extern __shared__ float2 scratch[];  // [kSmallThreads * VEC] | the slice's channels | its groups
+  const int slice = l.columns * VEC, group_channels = channels / groups, slice_groups = slice / group_channels;
+  float2 *sums = scratch + kSmallThreads * VEC, *stats = sums + slice;
+  const int tid = threadIdx.x, row = tid / l.columns;
+  const int first0 = blockIdx.x * slice, own = tid % l.columns * VEC, first = first0 + own;
+  const int group0 = first0 / group_channels;
+  const bool active = row < l.row_threads;
+  const int64_t step = (int64_t)l.row_threads * channels;
+  double total_a = 0.0, total_b = 0.0;  // backward: thread c < slice adds up channel c over the samples
+  const int64_t s0 = BACKWARD ? 0 : blockIdx.y, s1 = BACKWARD ? r.samples : s0 + 1;
+  for (int64_t sample = s0; sample < s1; ++sample) {
+    const int64_t begin = sampleStart(r, sample), end = sampleStart(r, sample + 1);
+    const int rows = end > begin ? (int)(end - begin) : 0;
+    const T *from0 = x + (begin + row) * channels + first;
+    const T *grad0 = BACKWARD ? dy + (begin + row) * channels + first : from0;
+    Two a[kPairs], b[kPairs], minus_k[kPairs];
+    Norm<VEC, UNIFORM> c;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float xhat = normalised(c, j, toFloat(p[u].v[j]));
-          const float du = activateGrad<ACT>(toFloat(g[u].v[j]), affine(c, j, xhat));
-          g[u].v[j] = fromFloat<T>((du * c.gamma[j] - m1[j] - xhat * m2[j]) * c.rstd[j]);
+    for (int j = 0; j < kPairs; ++j) a[j] = b[j] = minus_k[j] = two(0.0f, 0.0f);
+    if (active && rows > 0) {
+      if (BACKWARD) {
+        loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, group_channels);
+      } else {
+        Values<T, VEC> k;
+        k.load(x + begin * channels + first);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) minus_k[j] = k.pair(j) * two(-1.0f, -1.0f);
+      }
+      const T *from = from0, *grad = grad0;
+#pragma unroll 2
+      for (int i = row; i < rows; i += l.row_threads, from += step, grad += step) {
+        Values<T, VEC> v, g;
+        v.load(from);
+        if (BACKWARD) g.load(grad);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          if (BACKWARD) {
+            const Two xh = c.xhat(j, v.pair(j));
+            const Two du = activateGrad<ACT>(g.pair(j), c.affine(j, xh));
+            a[j] = a[j] + du;
+            b[j] = fma(du, xh, b[j]);
+          } else {
+            const Two d = v.pair(j) + minus_k[j];
+            a[j] = a[j] + d;
+            b[j] = fma(d, d, b[j]);
+          }
         }
-        storePack<VEC>(dx + (i + u * row_threads) * channels + first, g[u]);
       }
     }
-    at = stop;
+    joinRowThreads<VEC, kSmallThreads>(a, b, l, scratch, [&](int ch, float2 v) { sums[ch] = v; });
+    __syncthreads();
+    if (BACKWARD) {
+      if (tid < slice) {  // (slice <= kSmallThreads)
+        total_a += sums[tid].x;
+        total_b += sums[tid].y;
+      }
+    }
+    for (int q = tid; q < slice_groups; q += kSmallThreads) {
+      double u = 0.0, w = 0.0, ref = 0.0;
+      for (int i = 0; i < group_channels; ++i) {
+        const int ch = q * group_channels + i;
+        const float2 v = sums[ch];
+        if (BACKWARD) {
+          const double gamma = weight ? (double)loadAffine<T>(weight, float_affine, first0 + ch) : 1.0;
+          u += gamma * v.x;
+          w += gamma * v.y;
+        } else if (rows > 0) {  // (sum, squares) about the channel's first value
+          const double off = (double)v.x / rows, m = (double)toFloat(x[begin * channels + first0 + ch]) + off;
+          if (i == 0) ref = m;
+          const double squares = (double)v.y - (double)v.x * off;
+          u += m - ref;
+          w += (squares < 0.0 ? 0.0 : squares) + rows * (m - ref) * (m - ref);  // (NaN stays)
+        }
+      }
+      const double n = (double)(rows > 0 ? rows : 1) * group_channels;
+      if (BACKWARD) {
+        stats[q] = make_float2((float)(u / n), (float)(w / n));
+      } else {
+        const double off = u / group_channels;
+        double var = w / n - off * off;
+        var = var < 0.0 ? 0.0 : var;
+        const float m = (float)(ref + off), s = (float)(1.0 / sqrt(var + (double)epsilon));
+        stats[q] = make_float2(m, s);
+        mean[sample * groups + group0 + q] = m;
+        rstd[sample * groups + group0 + q] = s;
+      }
+    }
+    __syncthreads();
+    if (active && rows > 0) {
+      Two minus_m1[kGroups], minus_m2[kGroups];
+      auto group = [&](int j, auto value) {
+        return ofPair<UNIFORM ? 2 : VEC>(own, j, [&](int ch) { return value(stats[(UNIFORM ? own : ch) / group_channels]); });
+      };
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+        const Two first_stat = group(j, [](float2 v) { return -v.x; });
+        if (BACKWARD) {
+          minus_m1[j] = first_stat;
+          minus_m2[j] = group(j, [](float2 v) { return -v.y; });
+        } else {
+          c.minus_mean[j] = first_stat;
+          c.rstd[j] = group(j, [](float2 v) { return v.y; });
+        }
+      }
+      if (!BACKWARD) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          c.gamma[j] = ofPair<VEC>(first, j, [&](int ch) { return weight ? loadAffine<T>(weight, float_affine, ch) : 1.0f; });
+          c.beta[j] = ofPair<VEC>(first, j, [&](int ch) { return bias ? loadAffine<T>(bias, float_affine, ch) : 0.0f; });
+        }
+      }
+      const T *from = from0, *grad = grad0;
+      T *to = out + (begin + row) * channels + first;
+#pragma unroll 2
+      for (int i = row; i < rows; i += l.row_threads, from += step, grad += step, to += step) {
+        Values<T, VEC> v, g;
+        v.load(from);
+        if (BACKWARD) g.load(grad);
+        Two o[kPairs];
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const int q = UNIFORM ? 0 : j;
+          const Two xh = c.xhat(j, v.pair(j));
+          if (BACKWARD) {
+            const Two du = activateGrad<ACT>(g.pair(j), c.affine(j, xh));
+            o[j] = fma(xh, minus_m2[q], fma(du, c.gamma[j], minus_m1[q])) * c.rstd[q];
+          } else {
+            o[j] = activate<ACT>(c.affine(j, xh));
+          }
+        }
+        Values<T, VEC>::store(to, o);
+      }
+    }
+  }
+  if (BACKWARD && weight_grad && tid < slice) {
+    storeAffineGrad<T>(bias_grad, float_affine_grad, first0 + tid, total_a);
+    storeAffineGrad<T>(weight_grad, float_affine_grad, first0 + tid, total_b);
+  }
+  if (active && (BACKWARD || blockIdx.y == 0)) {  // rows of no sample
+    const int64_t covered = sampleStart(r, r.samples);
+    for (int64_t i = covered + row; i < r.rows; i += l.row_threads) Values<T, VEC>::storeZero(out + i * channels + first);
   }
 }
 
@@ -512,7 +631,41 @@ double rowBytes(const NormProblem &p) {
   return (double)p.rows * p.channels * mluop::getSizeOfDataType(p.dtype);
 }
 
-template <typename T, int VEC>
+// The one-launch form: its slices' width in vectors, or 0 where the rows are too many for it.  Measured on 256 x 128
+// values of 2 samples: one launch 6 us against 15 us for the three.
+int sliceColumns(const NormProblem &p, const NormPlan &plan, bool backward) {
+  if (plan.vec == 1 || p.samples == 0) return 0;
+  const int group_channels = p.channels / p.groups;
+  const int columns = std::lcm(group_channels, plan.vec) / plan.vec;
+  if (columns * plan.vec > kSmallThreads || p.channels % (columns * plan.vec) != 0) return 0;
+  // rows of one block: backward all of them; forward a sample's (on average) and, of the rows of no sample, all there may be
+  const int64_t rows = backward ? p.rows : (p.rows + p.samples - 1) / p.samples;
+  const int64_t turns = kSmallThreads / columns * (int64_t)kSmallTurns;
+  if (rows > turns || p.rows > 16 * turns || p.samples > (backward ? 64 : 65535)) return 0;
+  return columns;
+}
+
+template <typename T, int VEC, bool UNIFORM, bool BACKWARD>
+cudaError_t launchSlices(const NormProblem &p, int columns, const void *output_grad, const void *input, const void *weight,
+                         const void *bias, float *mean, float *rstd, void *out, void *weight_grad, void *bias_grad,
+                         cudaStream_t stream) {
+  const Lanes l{columns, kSmallThreads / columns};
+  const int slice = columns * VEC;
+  const size_t smem = ((size_t)kSmallThreads * VEC + slice + slice / (p.channels / p.groups)) * sizeof(float2);
+  const dim3 grid((unsigned)(p.channels / slice), BACKWARD ? 1u : (unsigned)p.samples);
+  trace::Scope scope(BACKWARD ? "groupNormSliceKernel:backward" : "groupNormSliceKernel:forward", stream,
+                     (BACKWARD ? 3 : 2) * rowBytes(p));
+  auto kernel = p.activation == MLUOP_GROUP_NORM_ACT_RELU   ? sliceKernel<T, VEC, MLUOP_GROUP_NORM_ACT_RELU, UNIFORM, BACKWARD>
+                : p.activation == MLUOP_GROUP_NORM_ACT_SILU ? sliceKernel<T, VEC, MLUOP_GROUP_NORM_ACT_SILU, UNIFORM, BACKWARD>
+                                                            : sliceKernel<T, VEC, MLUOP_GROUP_NORM_ACT_NONE, UNIFORM, BACKWARD>;
+  const Rows r{p.rows, p.samples, p.sample_rows, 0, p.sample_ends};
+  kernel<<<grid, kSmallThreads, smem, stream>>>(static_cast<const T *>(output_grad), static_cast<const T *>(input), weight,
+                                                bias, p.float_affine, mean, rstd, r, p.channels, p.groups, l, p.epsilon,
+                                                static_cast<T *>(out), weight_grad, bias_grad, p.float_affine_grad);
+  return cudaGetLastError();
+}
+
+template <typename T, int VEC, bool UNIFORM>
 cudaError_t forward(const NormProblem &p, const NormPlan &plan, const void *input, const void *weight,
                     const void *bias, void *workspace, void *output, float *mean, float *rstd, cudaStream_t stream) {
   char *base = scratchBase(workspace);
@@ -520,12 +673,12 @@ cudaError_t forward(const NormProblem &p, const NormPlan &plan, const void *inpu
   const T *x = static_cast<const T *>(input);
   T *y = static_cast<T *>(output);
   const Rows r = rowsOf(p, plan);
+  const Lanes l{plan.column_threads, plan.row_threads};
   const dim3 grid((unsigned)plan.blocks, (unsigned)plan.column_tiles);
-  const size_t smem = (size_t)plan.column_threads * plan.row_threads * VEC * sizeof(float2);
+  const size_t smem = (size_t)kThreads * VEC * sizeof(float2);
   {
     trace::Scope scope("groupNormStatisticsKernel", stream, rowBytes(p));
-    statisticsKernel<T, VEC><<<grid, kThreads, smem, stream>>>(x, r, p.channels, plan.column_threads,
-                                                               plan.row_threads, partial);
+    statisticsKernel<T, VEC><<<grid, kThreads, smem, stream>>>(x, r, p.channels, l, partial);
   }
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
@@ -537,15 +690,14 @@ cudaError_t forward(const NormProblem &p, const NormPlan &plan, const void *inpu
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   trace::Scope scope("groupNormNormaliseKernel", stream, 2 * rowBytes(p));
-  auto kernel = p.activation == MLUOP_GROUP_NORM_ACT_RELU   ? normaliseKernel<T, VEC, MLUOP_GROUP_NORM_ACT_RELU>
-                : p.activation == MLUOP_GROUP_NORM_ACT_SILU ? normaliseKernel<T, VEC, MLUOP_GROUP_NORM_ACT_SILU>
-                                                            : normaliseKernel<T, VEC, MLUOP_GROUP_NORM_ACT_NONE>;
-  kernel<<<grid, kThreads, 0, stream>>>(x, weight, bias, p.float_affine, mean, rstd, r, p.channels, p.groups,
-                                        plan.column_threads, plan.row_threads, y);
+  auto kernel = p.activation == MLUOP_GROUP_NORM_ACT_RELU   ? normaliseKernel<T, VEC, MLUOP_GROUP_NORM_ACT_RELU, UNIFORM>
+                : p.activation == MLUOP_GROUP_NORM_ACT_SILU ? normaliseKernel<T, VEC, MLUOP_GROUP_NORM_ACT_SILU, UNIFORM>
+                                                            : normaliseKernel<T, VEC, MLUOP_GROUP_NORM_ACT_NONE, UNIFORM>;
+  kernel<<<grid, kThreads, 0, stream>>>(x, weight, bias, p.float_affine, mean, rstd, r, p.channels, p.groups, l, y);
   return cudaGetLastError();
 }
 
-template <typename T, int VEC, int ACT>
+template <typename T, int VEC, bool UNIFORM, int ACT>
 cudaError_t backward(const NormProblem &p, const NormPlan &plan, const void *output_grad, const void *input,
                      const void *weight, const void *bias, const float *mean, const float *rstd, void *workspace,
                      void *input_grad, void *weight_grad, void *bias_grad, cudaStream_t stream) {
@@ -555,13 +707,13 @@ cudaError_t backward(const NormProblem &p, const NormPlan &plan, const void *out
   float2 *group_means = reinterpret_cast<float2 *>(base + plan.group_means);
   const T *dy = static_cast<const T *>(output_grad), *x = static_cast<const T *>(input);
   const Rows r = rowsOf(p, plan);
+  const Lanes l{plan.column_threads, plan.row_threads};
   const dim3 grid((unsigned)plan.blocks, (unsigned)plan.column_tiles);
-  const size_t smem = (size_t)plan.column_threads * plan.row_threads * VEC * sizeof(float2);
+  const size_t smem = (size_t)kThreads * VEC * sizeof(float2);
   {
     trace::Scope scope("groupNormGradSumsKernel", stream, 2 * rowBytes(p));
-    gradSumsKernel<T, VEC, ACT><<<grid, kThreads, smem, stream>>>(dy, x, weight, bias, p.float_affine, mean, rstd, r,
-                                                                  p.channels, p.groups, plan.column_threads,
-                                                                  plan.row_threads, partial);
+    gradSumsKernel<T, VEC, ACT, UNIFORM><<<grid, kThreads, smem, stream>>>(dy, x, weight, bias, p.float_affine, mean, rstd,
+                                                                           r, p.channels, p.groups, l, partial);
   }
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
@@ -573,20 +725,32 @@ cudaError_t backward(const NormProblem &p, const NormPlan &plan, const void *out
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   trace::Scope scope("groupNormInputGradKernel", stream, 3 * rowBytes(p));
-  inputGradKernel<T, VEC, ACT><<<grid, kThreads, 0, stream>>>(
-      dy, x, weight, bias, p.float_affine, mean, rstd, sample_sums, group_means, r, p.channels, p.groups,
-      plan.column_threads, plan.row_threads, static_cast<T *>(input_grad), weight_grad, bias_grad,
-      p.float_affine_grad);
+  inputGradKernel<T, VEC, ACT, UNIFORM><<<grid, kThreads, 0, stream>>>(
+      dy, x, weight, bias, p.float_affine, mean, rstd, sample_sums, group_means, r, p.channels, p.groups, l,
+      static_cast<T *>(input_grad), weight_grad, bias_grad, p.float_affine_grad);
   return cudaGetLastError();
 }
 
-template <typename T, int VEC, typename... Args>
+template <typename T, int VEC, bool UNIFORM, typename... Args>
 cudaError_t backwardAct(const NormProblem &p, Args... args) {
   switch (p.activation) {
-    case MLUOP_GROUP_NORM_ACT_RELU: return backward<T, VEC, MLUOP_GROUP_NORM_ACT_RELU>(p, args...);
-    case MLUOP_GROUP_NORM_ACT_SILU: return backward<T, VEC, MLUOP_GROUP_NORM_ACT_SILU>(p, args...);
-    default: return backward<T, VEC, MLUOP_GROUP_NORM_ACT_NONE>(p, args...);
+    case MLUOP_GROUP_NORM_ACT_RELU: return backward<T, VEC, UNIFORM, MLUOP_GROUP_NORM_ACT_RELU>(p, args...);
+    case MLUOP_GROUP_NORM_ACT_SILU: return backward<T, VEC, UNIFORM, MLUOP_GROUP_NORM_ACT_SILU>(p, args...);
+    default: return backward<T, VEC, UNIFORM, MLUOP_GROUP_NORM_ACT_NONE>(p, args...);
   }
+}
+
+// Vectors of 16 bytes whose channels lie in one group, such vectors across groups, or single values.
+template <typename T, int VEC, typename... Args>
+cudaError_t forwardType(const NormProblem &p, const NormPlan &plan, Args... args) {
+  if (plan.vec == 1) return forward<T, 1, true>(p, plan, args...);
+  return p.channels / p.groups % VEC == 0 ? forward<T, VEC, true>(p, plan, args...) : forward<T, VEC, false>(p, plan, args...);
+}
+template <typename T, int VEC, typename... Args>
+cudaError_t backwardType(const NormProblem &p, const NormPlan &plan, Args... args) {
+  if (plan.vec == 1) return backwardAct<T, 1, true>(p, plan, args...);
+  return p.channels / p.groups % VEC == 0 ? backwardAct<T, VEC, true>(p, plan, args...)
+                                          : backwardAct<T, VEC, false>(p, plan, args...);
 }
 
 bool aligned16(const void *p) { return reinterpret_cast<size_t>(p) % 16 == 0; }
@@ -601,8 +765,9 @@ NormPlan planNorm(const NormProblem &p, bool backward, bool vectors) {
   plan.column_threads = std::min(columns, kThreads);
   plan.column_tiles = (columns + plan.column_threads - 1) / plan.column_threads;
   plan.row_threads = kThreads / plan.column_threads;
-  // six blocks per SM over all column tiles, and at least one unrolled turn for each block
-  const int64_t wanted = std::max<int64_t>(1, (int64_t)6 * p.sm_count / plan.column_tiles);
+  // as many blocks as run at a time (four to an SM forward, three backward), so that each has long runs of rows, and at
+  // least one unrolled turn for each block
+  const int64_t wanted = std::max<int64_t>(1, (int64_t)(backward ? 3 : 4) * p.sm_count / plan.column_tiles);
   const int64_t turn = (int64_t)kUnroll * plan.row_threads;
   plan.block_rows = std::max<int64_t>(1, (p.rows + wanted - 1) / wanted);
   plan.block_rows = (plan.block_rows + turn - 1) / turn * turn;
@@ -618,31 +783,50 @@ size_t normWorkspaceBytes(const NormProblem &p, bool backward) {
   return std::max(planNorm(p, backward, true).total, planNorm(p, backward, false).total);
 }
 
+namespace {
+
+template <typename T, int VEC>
+cudaError_t runForward(const NormProblem &p, const void *input, const void *weight, const void *bias, void *workspace,
+                       void *output, float *mean, float *rstd, cudaStream_t stream) {
+  const NormPlan plan = planNorm(p, false, aligned16(input) && aligned16(output));
+  if (const int columns = sliceColumns(p, plan, false)) {
+    auto launch = p.channels / p.groups % VEC == 0 ? launchSlices<T, VEC, true, false> : launchSlices<T, VEC, false, false>;
+    return launch(p, columns, nullptr, input, weight, bias, mean, rstd, output, nullptr, nullptr, stream);
+  }
+  return forwardType<T, VEC>(p, plan, input, weight, bias, workspace, output, mean, rstd, stream);
+}
+
+template <typename T, int VEC>
+cudaError_t runBackward(const NormProblem &p, const void *output_grad, const void *input, const void *weight,
+                        const void *bias, const float *mean, const float *rstd, void *workspace, void *input_grad,
+                        void *weight_grad, void *bias_grad, cudaStream_t stream) {
+  const NormPlan plan = planNorm(p, true, aligned16(output_grad) && aligned16(input) && aligned16(input_grad));
+  if (const int columns = sliceColumns(p, plan, true)) {
+    auto launch = p.channels / p.groups % VEC == 0 ? launchSlices<T, VEC, true, true> : launchSlices<T, VEC, false, true>;
+    return launch(p, columns, output_grad, input, weight, bias, const_cast<float *>(mean), const_cast<float *>(rstd),
+                  input_grad, weight_grad, bias_grad, stream);
+  }
+  return backwardType<T, VEC>(p, plan, output_grad, input, weight, bias, mean, rstd, workspace, input_grad, weight_grad,
+                              bias_grad, stream);
+}
+
+}  // namespace
+
 cudaError_t launchNormForward(const NormProblem &p, const void *input, const void *weight, const void *bias,
                               void *workspace, void *output, float *mean, float *rstd, cudaStream_t stream) {
-  const NormPlan plan = planNorm(p, false, aligned16(input) && aligned16(output));
-#define MLUOP_FORWARD(T, VEC) forward<T, VEC>(p, plan, input, weight, bias, workspace, output, mean, rstd, stream)
-  switch (p.dtype) {
-    case MLUOP_DTYPE_FLOAT: return plan.vec == 4 ? MLUOP_FORWARD(float, 4) : MLUOP_FORWARD(float, 1);
-    case MLUOP_DTYPE_HALF: return plan.vec == 8 ? MLUOP_FORWARD(__half, 8) : MLUOP_FORWARD(__half, 1);
-    default: return plan.vec == 8 ? MLUOP_FORWARD(__nv_bfloat16, 8) : MLUOP_FORWARD(__nv_bfloat16, 1);
-  }
-#undef MLUOP_FORWARD
+  auto run = p.dtype == MLUOP_DTYPE_FLOAT ? runForward<float, 4>
+             : p.dtype == MLUOP_DTYPE_HALF ? runForward<__half, 8>
+                                           : runForward<__nv_bfloat16, 8>;
+  return run(p, input, weight, bias, workspace, output, mean, rstd, stream);
 }
 
 cudaError_t launchNormBackward(const NormProblem &p, const void *output_grad, const void *input, const void *weight,
                                const void *bias, const float *mean, const float *rstd, void *workspace,
                                void *input_grad, void *weight_grad, void *bias_grad, cudaStream_t stream) {
-  const NormPlan plan = planNorm(p, true, aligned16(output_grad) && aligned16(input) && aligned16(input_grad));
-#define MLUOP_BACKWARD(T, VEC)                                                                                    \
-  backwardAct<T, VEC>(p, plan, output_grad, input, weight, bias, mean, rstd, workspace, input_grad, weight_grad, \
-                      bias_grad, stream)
-  switch (p.dtype) {
-    case MLUOP_DTYPE_FLOAT: return plan.vec == 4 ? MLUOP_BACKWARD(float, 4) : MLUOP_BACKWARD(float, 1);
-    case MLUOP_DTYPE_HALF: return plan.vec == 8 ? MLUOP_BACKWARD(__half, 8) : MLUOP_BACKWARD(__half, 1);
-    default: return plan.vec == 8 ? MLUOP_BACKWARD(__nv_bfloat16, 8) : MLUOP_BACKWARD(__nv_bfloat16, 1);
-  }
-#undef MLUOP_BACKWARD
+  auto run = p.dtype == MLUOP_DTYPE_FLOAT ? runBackward<float, 4>
+             : p.dtype == MLUOP_DTYPE_HALF ? runBackward<__half, 8>
+                                           : runBackward<__nv_bfloat16, 8>;
+  return run(p, output_grad, input, weight, bias, mean, rstd, workspace, input_grad, weight_grad, bias_grad, stream);
 }
 
 }  // namespace group_norm_act

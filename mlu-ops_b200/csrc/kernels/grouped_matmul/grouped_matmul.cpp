@@ -82,23 +82,6 @@ mluOpStatus_t endsCheck(const std::string &api, const Problem &p, const mluOpTen
   return MLUOP_STATUS_SUCCESS;
 }
 
-// Where MLUOP_B200_CHECK_STATUS=1 asks for it and the stream is not being captured: waits for the work and reports an
-// error that it recorded.
-mluOpStatus_t checkIfRequested(const std::string &api, mluOpHandle_t handle) {
-  if (!mluop::checkStatusRequested()) return MLUOP_STATUS_SUCCESS;
-  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(handle->queue, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) {
-    (void)cudaGetLastError();
-    return MLUOP_STATUS_SUCCESS;
-  }
-  const cudaError_t err = cudaStreamSynchronize(handle->queue);
-  if (err != cudaSuccess) {
-    LOG(ERROR) << api << " execution failed: " << cudaGetErrorString(err);
-    return MLUOP_STATUS_EXECUTION_FAILED;
-  }
-  return mluop::takeStickyDeviceError(handle, api.c_str()) ? MLUOP_STATUS_EXECUTION_FAILED : MLUOP_STATUS_SUCCESS;
-}
-
 mluOpStatus_t run(const std::string &api, mluOpHandle_t handle, Problem &p, const void *a, const void *b,
                   const void *ends, void *c, void *workspace) {
   if (handle->host_only) {
@@ -107,11 +90,7 @@ mluOpStatus_t run(const std::string &api, mluOpHandle_t handle, Problem &p, cons
   }
   if (mluop::takeStickyDeviceError(handle, api.c_str())) return MLUOP_STATUS_EXECUTION_FAILED;
   mluop::DeviceGuard guard(handle);
-  p.sticky = nullptr;
-  if (cudaHostGetDevicePointer((void **)&p.sticky, handle->host_words + mluOpContext::kStickyWord, 0) != cudaSuccess) {
-    (void)cudaGetLastError();
-    p.sticky = nullptr;
-  }
+  p.sticky = mluop::stickyDeviceWord(handle);
   const int32_t *group_ends = static_cast<const int32_t *>(ends);
   const cudaError_t err =
       mluop::grouped_matmul::tensorCoresEligible(p, a, b, c)
@@ -121,7 +100,7 @@ mluOpStatus_t run(const std::string &api, mluOpHandle_t handle, Problem &p, cons
     LOG(ERROR) << api << " launch failed: " << cudaGetErrorString(err);
     return MLUOP_STATUS_EXECUTION_FAILED;
   }
-  return checkIfRequested(api, handle);
+  return mluop::reportIfRequested(handle, api.c_str());
 }
 
 }  // namespace
