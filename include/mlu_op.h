@@ -635,6 +635,7 @@ typedef enum {
  * epsilon > 0.  Statistics are held in float and combined in a fixed order:
  * results are reproducible run to run.  Descriptors are contiguous, every tensor
  * has fewer than 2^31 rows and C <= 65536.  output may be input (in place).
+ * The workspace query may answer 0; workspace may be NULL then.
  * Asynchronous on the handle's queue. */
 mluOpStatus_t MLUOP_WIN_API mluOpGetGroupNormActForwardWorkspaceSize(
     mluOpHandle_t handle, const mluOpTensorDescriptor_t input_desc,

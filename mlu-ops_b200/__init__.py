@@ -6,6 +6,7 @@ backbone driver can pass torch CUDA tensors.  Function and argument names
 follow the reference's C API.  There is no CPU fallback: if the library has not
 been built, loading raises.
 """
+import array
 import ctypes
 import os
 
@@ -800,9 +801,18 @@ def _new(like, shape, dtype):
     return like.new_empty(shape, dtype=dtype)
 
 
-def _workspace(like, nbytes):
+def _new_like(t):
     import torch
-    return _new(like, (nbytes,), torch.uint8)
+    return torch.empty_like(t) if _guards is None else _guards.empty(t.shape, t.dtype, t.device)
+
+
+def _workspace(like, nbytes):
+    """(tensor, address) of a workspace; (None, None) if none is needed."""
+    import torch
+    if nbytes == 0:
+        return None, None
+    t = _new(like, (nbytes,), torch.uint8)
+    return t, t.data_ptr()
 
 
 def _spec(t):
@@ -835,7 +845,7 @@ def group_norm_act_forward(handle, input, weight, bias, num_groups, epsilon=1e-5
     num_groups = int(num_groups)
     stats = ((input.shape[0] if sample_ends is None else sample_ends.shape[0]), num_groups)
     if out is None:
-        out = _new(input, input.shape, input.dtype)
+        out = _new_like(input)
     mean, rstd = _new(input, stats, torch.float32), _new(input, stats, torch.float32)
     p_y = _address(handle, "out", out)
     specs = lambda: [_spec(t) for t in (input, weight, bias, sample_ends, out)] + [(torch.float32, stats)]  # noqa: E731
@@ -845,11 +855,10 @@ def group_norm_act_forward(handle, input, weight, bias, num_groups, epsilon=1e-5
                                                lib().mluOpGetGroupNormActForwardWorkspaceSize(
                                                    handle.ptr, plan.d[0], plan.d[3], num_groups, ctypes.byref(size))))
     d_x, d_w, d_b, d_e, d_y, d_m = plan.d
-    workspace = _workspace(input, plan.workspace)
+    workspace, p_s = _workspace(input, plan.workspace)
     check("mluOpGroupNormActForward",
           lib().mluOpGroupNormActForward(handle.ptr, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, num_groups, epsilon, act,
-                                         workspace.data_ptr(), plan.workspace, d_y, p_y, d_m, mean.data_ptr(), d_m,
-                                         rstd.data_ptr()))
+                                         p_s, plan.workspace, d_y, p_y, d_m, mean.data_ptr(), d_m, rstd.data_ptr()))
     return out, mean, rstd
 
 
@@ -871,7 +880,7 @@ def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd
     p_m, p_r = _address(handle, "mean", mean), _address(handle, "rstd", rstd)
     num_groups = int(num_groups)
     if out is None:
-        out = _new(input, input.shape, input.dtype)
+        out = _new_like(input)
     p_o = _address(handle, "out", out)
     weight_grad = bias_grad = p_wg = p_bg = None
     if affine_grad:
@@ -885,11 +894,11 @@ def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd
                                                lib().mluOpGetGroupNormActBackwardWorkspaceSize(
                                                    handle.ptr, plan.d[1], plan.d[4], num_groups, ctypes.byref(size))))
     d_g, d_x, d_w, d_b, d_e, d_m, d_r, d_o, d_wg, d_bg = plan.d
-    workspace = _workspace(input, plan.workspace)
+    workspace, p_s = _workspace(input, plan.workspace)
     check("mluOpGroupNormActBackward",
           lib().mluOpGroupNormActBackward(handle.ptr, d_g, p_g, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, d_m, p_m, d_r,
-                                          p_r, num_groups, act, workspace.data_ptr(), plan.workspace, d_o, p_o, d_wg,
-                                          p_wg, d_bg, p_bg))
+                                          p_r, num_groups, act, p_s, plan.workspace, d_o, p_o, d_wg, p_wg, d_bg,
+                                          p_bg))
     return out, weight_grad, bias_grad
 
 
@@ -897,7 +906,9 @@ SCALE_BLOCK = 256  # consecutive elements of an 8-bit optimiser state that share
 
 
 def _addresses(tensors):
-    return (_vp * len(tensors))(*[t.data_ptr() for t in tensors])
+    """A C array of the tensors' addresses."""
+    import torch
+    return array.array("Q", map(torch.Tensor.data_ptr, tensors))
 
 
 class MultiTensorAdamW:
@@ -963,20 +974,22 @@ class MultiTensorAdamW:
             return
         if self.device != handle.device:
             raise ValueError("the tensors lie on device %s, the handle on CUDA device %d" % (self.device, handle.device))
-        dtype = grads[0].dtype
-        for g, n in zip(grads, self.numels):
-            if g.numel() != n or g.dtype is not dtype or g.get_device() != self.device or not g.is_contiguous():
-                raise ValueError("gradients are dense, of one type, on the parameters' device and of their sizes")
+        dtype, of = grads[0].dtype, torch.Tensor  # (mapped methods: a step of many small tensors is mostly this)
+        if (list(map(of.numel, grads)) != self.numels or {g.dtype for g in grads} != {dtype}
+                or set(map(of.get_device, grads)) != {self.device} or not all(map(of.is_contiguous, grads))):
+            raise ValueError("gradients are dense, of one type, on the parameters' device and of their sizes")
         for name, t, n in (("grad_scale", grad_scale, 1), ("schedule", schedule, 3)):
             if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.get_device() != self.device
                                   or not t.is_contiguous()):
                 raise ValueError("%s is a dense float32 tensor of %d element(s) on the parameters' device" % (name, n))
+        grad_p = _addresses(grads)
         check("mluOpMultiTensorAdamW",
               lib().mluOpMultiTensorAdamW(handle.ptr, _dtype_code(self.dtype), _dtype_code(dtype),
                                           DTYPE_UINT8 if self.eight_bit else DTYPE_FLOAT, len(self.params),
-                                          self._numel_p, self._param_p, _addresses(grads), self._m_p, self._v_p,
-                                          *self._scale_p, lr, betas[0], betas[1], epsilon, weight_decay, int(step),
-                                          _ptr(grad_scale), _ptr(schedule)))
+                                          self._numel_p, self._param_p.buffer_info()[0], grad_p.buffer_info()[0],
+                                          self._m_p.buffer_info()[0], self._v_p.buffer_info()[0],
+                                          *[p and p.buffer_info()[0] for p in self._scale_p], lr, betas[0], betas[1],
+                                          epsilon, weight_decay, int(step), _ptr(grad_scale), _ptr(schedule)))
 
 
 def grouped_matmul_forward(handle, input, weight, group_ends, out=None):
@@ -1035,8 +1048,8 @@ def grouped_matmul_backward_weight(handle, input, output_grad, group_ends, dtype
                                                lib().mluOpGetGroupedMatMulBackwardWeightWorkspaceSize(
                                                    handle.ptr, plan.d[0], plan.d[1], plan.d[3], ctypes.byref(size))))
     d_x, d_g, d_e, d_w = plan.d
-    workspace = _workspace(input, plan.workspace)
+    workspace, p_s = _workspace(input, plan.workspace)
     check("mluOpGroupedMatMulBackwardWeight",
-          lib().mluOpGroupedMatMulBackwardWeight(handle.ptr, d_x, p_x, d_g, p_g, d_e, p_e, workspace.data_ptr(),
-                                                 plan.workspace, d_w, p_w))
+          lib().mluOpGroupedMatMulBackwardWeight(handle.ptr, d_x, p_x, d_g, p_g, d_e, p_e, p_s, plan.workspace, d_w,
+                                                 p_w))
     return out

@@ -133,7 +133,7 @@ mluOpStatus_t workspaceSize(const std::string &api, mluOpHandle_t handle, const 
 mluOpStatus_t workspaceCheck(const std::string &api, const NormProblem &p, bool backward, const void *workspace,
                              size_t workspace_size) {
   const size_t need = mluop::group_norm_act::normWorkspaceBytes(p, backward);
-  if (workspace == nullptr || workspace_size < need) {
+  if ((workspace == nullptr && need > 0) || workspace_size < need) {
     LOG(ERROR) << api << " workspace of " << workspace_size << " bytes is smaller than the " << need
                << " bytes that the query reports.";
     return MLUOP_STATUS_BAD_PARAM;

@@ -631,19 +631,22 @@ double rowBytes(const NormProblem &p) {
   return (double)p.rows * p.channels * mluop::getSizeOfDataType(p.dtype);
 }
 
-// The one-launch form: its slices' width in vectors, or 0 where the rows are too many for it.  Measured on 256 x 128
-// values of 2 samples: one launch 6 us against 15 us for the three.
-int sliceColumns(const NormProblem &p, const NormPlan &plan, bool backward) {
-  if (plan.vec == 1 || p.samples == 0) return 0;
+}  // namespace
+
+// Measured on 256 x 128 values of 2 samples: one launch 6 us against 15 us for the three.
+int sliceColumns(const NormProblem &p, int vec, bool backward) {
+  if (p.samples == 0) return 0;
   const int group_channels = p.channels / p.groups;
-  const int columns = std::lcm(group_channels, plan.vec) / plan.vec;
-  if (columns * plan.vec > kSmallThreads || p.channels % (columns * plan.vec) != 0) return 0;
+  const int columns = std::lcm(group_channels, vec) / vec;
+  if (columns * vec > kSmallThreads || p.channels % (columns * vec) != 0) return 0;
   // rows of one block: backward all of them; forward a sample's (on average) and, of the rows of no sample, all there may be
   const int64_t rows = backward ? p.rows : (p.rows + p.samples - 1) / p.samples;
   const int64_t turns = kSmallThreads / columns * (int64_t)kSmallTurns;
   if (rows > turns || p.rows > 16 * turns || p.samples > (backward ? 64 : 65535)) return 0;
   return columns;
 }
+
+namespace {
 
 template <typename T, int VEC, bool UNIFORM, bool BACKWARD>
 cudaError_t launchSlices(const NormProblem &p, int columns, const void *output_grad, const void *input, const void *weight,
@@ -780,6 +783,9 @@ NormPlan planNorm(const NormProblem &p, bool backward, bool vectors) {
 }
 
 size_t normWorkspaceBytes(const NormProblem &p, bool backward) {
+  // whichever way the tensors are aligned, the one-launch form needs none
+  const int wide = 16 / (int)mluop::getSizeOfDataType(p.dtype);
+  if (sliceColumns(p, 1, backward) && (p.channels % wide != 0 || sliceColumns(p, wide, backward))) return 0;
   return std::max(planNorm(p, backward, true).total, planNorm(p, backward, false).total);
 }
 
@@ -789,8 +795,10 @@ template <typename T, int VEC>
 cudaError_t runForward(const NormProblem &p, const void *input, const void *weight, const void *bias, void *workspace,
                        void *output, float *mean, float *rstd, cudaStream_t stream) {
   const NormPlan plan = planNorm(p, false, aligned16(input) && aligned16(output));
-  if (const int columns = sliceColumns(p, plan, false)) {
-    auto launch = p.channels / p.groups % VEC == 0 ? launchSlices<T, VEC, true, false> : launchSlices<T, VEC, false, false>;
+  if (const int columns = sliceColumns(p, plan.vec, false)) {
+    auto launch = plan.vec == 1                        ? launchSlices<T, 1, true, false>
+                  : p.channels / p.groups % VEC == 0 ? launchSlices<T, VEC, true, false>
+                                                     : launchSlices<T, VEC, false, false>;
     return launch(p, columns, nullptr, input, weight, bias, mean, rstd, output, nullptr, nullptr, stream);
   }
   return forwardType<T, VEC>(p, plan, input, weight, bias, workspace, output, mean, rstd, stream);
@@ -801,8 +809,10 @@ cudaError_t runBackward(const NormProblem &p, const void *output_grad, const voi
                         const void *bias, const float *mean, const float *rstd, void *workspace, void *input_grad,
                         void *weight_grad, void *bias_grad, cudaStream_t stream) {
   const NormPlan plan = planNorm(p, true, aligned16(output_grad) && aligned16(input) && aligned16(input_grad));
-  if (const int columns = sliceColumns(p, plan, true)) {
-    auto launch = p.channels / p.groups % VEC == 0 ? launchSlices<T, VEC, true, true> : launchSlices<T, VEC, false, true>;
+  if (const int columns = sliceColumns(p, plan.vec, true)) {
+    auto launch = plan.vec == 1                        ? launchSlices<T, 1, true, true>
+                  : p.channels / p.groups % VEC == 0 ? launchSlices<T, VEC, true, true>
+                                                     : launchSlices<T, VEC, false, true>;
     return launch(p, columns, output_grad, input, weight, bias, const_cast<float *>(mean), const_cast<float *>(rstd),
                   input_grad, weight_grad, bias_grad, stream);
   }

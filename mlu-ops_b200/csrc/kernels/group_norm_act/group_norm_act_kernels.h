@@ -37,6 +37,8 @@ struct NormPlan {
   size_t partial, sample_sums, group_means, total;
 };
 
+// The one-launch form for few rows: the width of its slices in vectors of `vec` channels, or 0 where it does not apply.
+int sliceColumns(const NormProblem &p, int vec, bool backward);
 NormPlan planNorm(const NormProblem &p, bool backward, bool vectors);
 size_t normWorkspaceBytes(const NormProblem &p, bool backward);
 

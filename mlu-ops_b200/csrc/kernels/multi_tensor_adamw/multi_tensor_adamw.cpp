@@ -86,7 +86,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW(
   mluop::multi_tensor_adamw::AdamWProblem p{param_dtype, grad_dtype,    state_8bit,       tensor_num, element_num,
                                             param,       grad,          exp_avg,          exp_avg_sq, exp_avg_scale,
                                             exp_avg_sq_scale, lr,       beta1,            beta2,      epsilon,
-                                            weight_decay, step,         grad_scale,       schedule};
+                                            weight_decay, step,         grad_scale,       schedule, handle->sm_count};
   const cudaError_t err = mluop::multi_tensor_adamw::launchMultiTensorAdamW(p, handle->queue);
   if (err != cudaSuccess) {
     LOG(ERROR) << api << " launch failed: " << cudaGetErrorString(err);

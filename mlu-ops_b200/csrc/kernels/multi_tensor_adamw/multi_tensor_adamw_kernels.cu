@@ -9,12 +9,17 @@
 // for bfloat16 parameters with 8-bit states.  One launch serves up to kMaxTensors
 // tensors: their pointers travel as a kernel argument (29 KB of the 32 KB that an
 // argument list may have), so nothing is copied to the device and a captured graph
-// carries them.  Tensors are cut into chunks of 4096 elements, a block each; a block
-// finds its tensor by bisection of the chunk counts.
+// carries them.  Tensors are cut into chunks of 1024 to 4096 elements, a block each; a
+// block finds its tensor by bisection of the chunk counts.
 //
-// The order of the roundings is fixed (no contraction into fused multiply-adds): the
-// values before quantisation are then the same on any path through this file, and
-// two elements that tie in 8 bits tie everywhere.
+// Float states: the roundings are those of the formula evaluated step by step.
+// 8-bit states: with 10 bytes an element the arithmetic is what has to be short.  It
+// runs on pairs of floats, with fused multiply-adds, and with the approximate square
+// root and reciprocal (2^-22 of the value; the states are rounded to 2^-4 of it
+// afterwards): 34 instructions an element.  Correctly rounded single operations took
+// 296 us for 10^8 bfloat16 elements, this form 177 us (1.0 GB: 5.7 TB/s).  One block
+// of 256 a warp and five blocks of threads an SM; two or four blocks a warp, their
+// loads ahead of their use, took 189 and 250 us.
 //
 // 8-bit states: blocks of 256 consecutive elements share a float scale, one warp
 // takes one block (8 elements a lane), its largest magnitude by one warp reduction.
@@ -32,6 +37,7 @@
 #include <cmath>
 
 #include "core/convert.cuh"
+#include "core/pair.cuh"
 #include "core/trace.h"
 #include "core/type.h"
 
@@ -41,7 +47,9 @@ namespace multi_tensor_adamw {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 4096;       // elements of one block; a multiple of kScaleBlock
+constexpr int kChunk = 4096;       // elements of one block, float states
+constexpr int kSmallChunk = 1024;  // the same where chunks of 4096 would not fill the SMs
+constexpr int kChunk8Bit = 2048;   // 8-bit states: a block of 256 for each warp
 constexpr int kMaxTensors = 480;   // tensors of one launch
 constexpr float kCodeMax = 448.0f;  // largest e4m3 value
 constexpr float kSmallest = 1e-30f;  // below it a block is stored as zeros: 448 / x would leave the float range
@@ -105,12 +113,12 @@ __device__ __forceinline__ int findTensor(const TensorTable &t, int chunk) {
 
 __device__ __forceinline__ bool aligned16(const void *p) { return (reinterpret_cast<size_t>(p) & 15) == 0; }
 
-template <typename P, typename G>
+template <typename P, typename G, int CHUNK>
 __global__ void __launch_bounds__(kThreads) adamWKernel(const __grid_constant__ TensorTable t) {
   const int which = findTensor(t, blockIdx.x);
-  const int64_t begin = (int64_t)((int)blockIdx.x - t.first_chunk[which]) * kChunk;
+  const int64_t begin = (int64_t)((int)blockIdx.x - t.first_chunk[which]) * CHUNK;
   const int64_t left = t.n[which] - begin;
-  const int count = left < kChunk ? (int)left : kChunk;
+  const int count = left < CHUNK ? (int)left : CHUNK;
   P *param = static_cast<P *>(t.param[which]) + begin;
   const G *grad = static_cast<const G *>(t.grad[which]) + begin;
   float *exp_avg = static_cast<float *>(t.exp_avg[which]) + begin;
@@ -119,9 +127,9 @@ __global__ void __launch_bounds__(kThreads) adamWKernel(const __grid_constant__ 
   const bool scaled = t.grad_scale != nullptr;
   const float gs = scaled ? *t.grad_scale : 1.0f;
   const bool vectors = aligned16(param) && aligned16(grad) && aligned16(exp_avg) && aligned16(exp_avg_sq);
-  if (count == kChunk && vectors) {
+  if (count == CHUNK && vectors) {
     // 4 elements a thread and turn, all loads of the four turns in flight before the first use
-    constexpr int kTurns = kChunk / (4 * kThreads);
+    constexpr int kTurns = CHUNK / (4 * kThreads);
     Pack<4, P> p[kTurns];
     Pack<4, G> g[kTurns];
     Pack<4, float> m[kTurns], v[kTurns];
@@ -157,124 +165,193 @@ __global__ void __launch_bounds__(kThreads) adamWKernel(const __grid_constant__ 
   }
 }
 
+// 8-bit states.  A pair of codes as floats, and back.
+__device__ __forceinline__ Two fromCodes(unsigned short codes) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(codes, __NV_E4M3);
+  const float2 f = __half22float2(__half2(h));
+  return two(f.x, f.y);
+}
+__device__ __forceinline__ unsigned short toCodes(Two t) { return __nv_cvt_float2_to_fp8x2(split(t), __NV_SATFINITE, __NV_E4M3); }
+
+// Eight consecutive values as pairs.
+template <typename T>
+struct Eight {
+  static constexpr int kEach = 16 / sizeof(T), kVectors = 8 / kEach;
+  Values<T, kEach> v[kVectors];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) v[i].load(p + i * kEach);
+  }
+  __device__ __forceinline__ Two pair(int j) const { return v[j / (kEach / 2)].pair(j % (kEach / 2)); }
+  static __device__ __forceinline__ void store(T *p, const Two (&t)[4]) {
+    if constexpr (kVectors == 1) {
+      Values<T, kEach>::store(p, t);
+    } else {
+      Values<T, kEach>::store(p, {t[0], t[1]});
+      Values<T, kEach>::store(p + kEach, {t[2], t[3]});
+    }
+  }
+};
+
+// The larger of a and |b|; NaN if either is one.
+__device__ __forceinline__ float largest(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
+
+struct Pairs {
+  Two beta1, one_minus_beta1, beta2, one_minus_beta2, epsilon, decay, root_scale, minus_step;
+  __device__ __forceinline__ explicit Pairs(const Constants &c)
+      : beta1(two(c.beta1, c.beta1)),
+        one_minus_beta1(two(c.one_minus_beta1, c.one_minus_beta1)),
+        beta2(two(c.beta2, c.beta2)),
+        one_minus_beta2(two(c.one_minus_beta2, c.one_minus_beta2)),
+        epsilon(two(c.epsilon, c.epsilon)),
+        decay(two(c.decay, c.decay)),
+        root_scale(two(c.root_scale, c.root_scale)),
+        minus_step(two(-c.step_size, -c.step_size)) {}
+};
+// Two elements: m and root (sqrt(v)) are updated in place.  Returns the new parameters.
+__device__ __forceinline__ Two updatePair(Two p, Two g, Two &m, Two &root, const Pairs &c) {
+  m = fma(g, c.one_minus_beta1, m * c.beta1);
+  float2 r = split(fma(g * g, c.one_minus_beta2, (root * root) * c.beta2));
+  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(r.x));
+  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(r.y));
+  root = two(r.x, r.y);
+  float2 d = split(fma(root, c.root_scale, c.epsilon));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.y));
+  return fma(m * two(d.x, d.y), c.minus_step, p * c.decay);
+}
+
 struct BlockScale {
   float scale, inverse;
 };
-// Scale of a block of 256 whose lanes hold `largest` as the bits of magnitudes (unsigned order; NaN is the
-// largest, so that a NaN reaches its whole block).
-__device__ __forceinline__ BlockScale blockScale(unsigned largest_bits) {
-  const float largest = __uint_as_float(__reduce_max_sync(0xffffffffu, largest_bits));
+// Scale of a block of 256 from the largest magnitude that each lane holds (a NaN, larger than any other by its bits,
+// reaches its whole block).
+__device__ __forceinline__ BlockScale blockScale(float lane_largest) {
+  const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lane_largest)));
   BlockScale s{0.0f, 0.0f};
-  if (!(largest < kSmallest)) {
-    s.inverse = __fdiv_rn(kCodeMax, largest);
-    s.scale = __fmul_rn(largest, 1.0f / kCodeMax);
+  if (!(most < kSmallest)) {
+    s.inverse = __fdiv_rn(kCodeMax, most);
+    s.scale = __fmul_rn(most, 1.0f / kCodeMax);
   }
   return s;
 }
-__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-__device__ __forceinline__ float rootCode(float root, float inverse) {
-  const float code = __fmul_rn(root, inverse);
-  return (root > 0.0f && inverse > 0.0f && code < kCodeTiny) ? kCodeTiny : code;
+__device__ __forceinline__ Two rootCodes(Two root, float inverse) {
+  const float2 r = split(root);
+  float2 code = split(root * two(inverse, inverse));
+  const float least = inverse > 0.0f ? kCodeTiny : 0.0f;
+  code.x = r.x > 0.0f ? fmaxf(code.x, least) : code.x;
+  code.y = r.y > 0.0f ? fmaxf(code.y, least) : code.y;
+  return two(code.x, code.y);
 }
-__device__ __forceinline__ float fromCode(unsigned char code) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3)));
-}
-__device__ __forceinline__ unsigned char toCode(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 
 template <typename P, typename G>
-__global__ void __launch_bounds__(kThreads) adamW8BitKernel(const __grid_constant__ TensorTable t) {
+__global__ void __launch_bounds__(kThreads, 5) adamW8BitKernel(const __grid_constant__ TensorTable t) {
   const int which = findTensor(t, blockIdx.x);
-  const int64_t begin = (int64_t)((int)blockIdx.x - t.first_chunk[which]) * kChunk;
+  const int64_t begin = (int64_t)((int)blockIdx.x - t.first_chunk[which]) * kChunk8Bit;
   const int64_t left = t.n[which] - begin;
-  const int count = left < kChunk ? (int)left : kChunk;
+  const int count = left < kChunk8Bit ? (int)left : kChunk8Bit;
   P *param = static_cast<P *>(t.param[which]) + begin;
   const G *grad = static_cast<const G *>(t.grad[which]) + begin;
   unsigned char *exp_avg = static_cast<unsigned char *>(t.exp_avg[which]) + begin;
   unsigned char *exp_avg_sq = static_cast<unsigned char *>(t.exp_avg_sq[which]) + begin;
   float *m_scales = t.exp_avg_scale[which] + begin / kScaleBlock;
   float *v_scales = t.exp_avg_sq_scale[which] + begin / kScaleBlock;
-  const Constants c = stepConstants(t);
-  const bool scaled = t.grad_scale != nullptr;
-  const float gs = scaled ? *t.grad_scale : 1.0f;
+  const Pairs c(stepConstants(t));
+  const float gs = t.grad_scale ? *t.grad_scale : 1.0f;
+  const Two scale_grad = two(gs, gs);
   const bool vectors = aligned16(param) && aligned16(grad) && aligned16(exp_avg) && aligned16(exp_avg_sq);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kWarps = kThreads / 32;
-  constexpr int kBlocks = kChunk / (int)kScaleBlock / kWarps;  // blocks of 256 a warp takes: 2
-  if (count == kChunk && vectors) {
-    Pack<8, P> p[kBlocks];
-    Pack<8, G> g[kBlocks];
-    Pack<8, unsigned char> mc[kBlocks], vc[kBlocks];
-    float ms[kBlocks], vs[kBlocks];
+  static_assert(kChunk8Bit == kWarps * kScaleBlock, "one block a warp");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (count == kChunk8Bit && vectors) {
+    const int block = warp, at = block * (int)kScaleBlock + lane * 8;
+    Eight<P> p;
+    Eight<G> g;
+    p.load(param + at);
+    g.load(grad + at);
+    const uint2 mc = *reinterpret_cast<const uint2 *>(exp_avg + at), vc = *reinterpret_cast<const uint2 *>(exp_avg_sq + at);
+    const float ms = m_scales[block], vs = v_scales[block];
+    Two m[4], root[4], next[4];
+    float m_max = 0.0f, v_max = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) {
-      const int block = i * kWarps + warp, at = block * (int)kScaleBlock + lane * 8;
-      p[i] = loadPack<8>(param + at);
-      g[i] = loadPack<8>(grad + at);
-      mc[i] = loadPack<8>(exp_avg + at);
-      vc[i] = loadPack<8>(exp_avg_sq + at);
-      ms[i] = m_scales[block];
-      vs[i] = v_scales[block];
+    for (int j = 0; j < 4; ++j) {
+      const unsigned mw = j < 2 ? mc.x : mc.y, vw = j < 2 ? vc.x : vc.y;
+      m[j] = fromCodes((unsigned short)(mw >> (j & 1) * 16)) * two(ms, ms);
+      root[j] = fromCodes((unsigned short)(vw >> (j & 1) * 16)) * two(vs, vs);
+      next[j] = updatePair(p.pair(j), g.pair(j) * scale_grad, m[j], root[j], c);
+      const float2 a = split(m[j]), b = split(root[j]);
+      m_max = largest(largest(m_max, a.x), a.y);
+      v_max = largest(largest(v_max, b.x), b.y);
     }
+    Eight<P>::store(param + at, next);
+    const BlockScale m_scale = blockScale(m_max), v_scale = blockScale(v_max);
+    unsigned short mo[4], vo[4];
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) {
-      const int block = i * kWarps + warp, at = block * (int)kScaleBlock + lane * 8;
-      float m[8], root[8];
-      unsigned m_max = 0u, v_max = 0u;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float gj = toFloat(g[i].v[j]);
-        if (scaled) gj = __fmul_rn(gj, gs);
-        m[j] = __fmul_rn(fromCode(mc[i].v[j]), ms[i]);
-        const float old_root = __fmul_rn(fromCode(vc[i].v[j]), vs[i]);
-        float v = __fmul_rn(old_root, old_root);
-        p[i].v[j] = fromFloat<P>(updateOne(toFloat(p[i].v[j]), gj, m[j], v, root[j], c));
-        m_max = max(m_max, magnitude(m[j]));
-        v_max = max(v_max, magnitude(root[j]));
-      }
-      const BlockScale m_scale = blockScale(m_max), v_scale = blockScale(v_max);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        mc[i].v[j] = toCode(__fmul_rn(m[j], m_scale.inverse));
-        vc[i].v[j] = toCode(rootCode(root[j], v_scale.inverse));
-      }
-      storePack<8>(param + at, p[i]);
-      storePack<8>(exp_avg + at, mc[i]);
-      storePack<8>(exp_avg_sq + at, vc[i]);
-      if (lane == 0) {
-        m_scales[block] = m_scale.scale;
-        v_scales[block] = v_scale.scale;
-      }
+    for (int j = 0; j < 4; ++j) {
+      mo[j] = toCodes(m[j] * two(m_scale.inverse, m_scale.inverse));
+      vo[j] = toCodes(rootCodes(root[j], v_scale.inverse));
+    }
+    *reinterpret_cast<uint2 *>(exp_avg + at) = make_uint2(mo[0] | (unsigned)mo[1] << 16, mo[2] | (unsigned)mo[3] << 16);
+    *reinterpret_cast<uint2 *>(exp_avg_sq + at) = make_uint2(vo[0] | (unsigned)vo[1] << 16, vo[2] | (unsigned)vo[3] << 16);
+    if (lane == 0) {
+      m_scales[block] = m_scale.scale;
+      v_scales[block] = v_scale.scale;
     }
     return;
   }
-  // a tensor's last chunk, or pointers that are not 16-byte aligned: element by element, lanes side by side
+  // A tensor's last chunk, or pointers that are not 16-byte aligned: element by element, lanes side by side.  A pair is
+  // elements 32 apart.
   const int blocks = (count + (int)kScaleBlock - 1) / (int)kScaleBlock;
   for (int block = warp; block < blocks; block += kWarps) {
     const float ms = m_scales[block], vs = v_scales[block];
-    float m[8], root[8];
-    unsigned m_max = 0u, v_max = 0u;
+    Two m[4], root[4];
+    float m_max = 0.0f, v_max = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int at = block * (int)kScaleBlock + j * 32 + lane;
-      m[j] = root[j] = 0.0f;
-      if (at < count) {
-        float gj = toFloat(grad[at]);
-        if (scaled) gj = __fmul_rn(gj, gs);
-        m[j] = __fmul_rn(fromCode(exp_avg[at]), ms);
-        const float old_root = __fmul_rn(fromCode(exp_avg_sq[at]), vs);
-        float v = __fmul_rn(old_root, old_root);
-        param[at] = fromFloat<P>(updateOne(toFloat(param[at]), gj, m[j], v, root[j], c));
-        m_max = max(m_max, magnitude(m[j]));
-        v_max = max(v_max, magnitude(root[j]));
+    for (int j = 0; j < 4; ++j) {
+      const int at0 = block * (int)kScaleBlock + 2 * j * 32 + lane, at1 = at0 + 32;
+      const bool in0 = at0 < count, in1 = at1 < count;
+      unsigned short mc = 0, vc = 0;
+      float p0 = 0.0f, p1 = 0.0f, g0 = 0.0f, g1 = 0.0f;
+      if (in0) {
+        mc = exp_avg[at0];
+        vc = exp_avg_sq[at0];
+        p0 = toFloat(param[at0]);
+        g0 = toFloat(grad[at0]);
       }
+      if (in1) {
+        mc |= (unsigned short)(exp_avg[at1] << 8);
+        vc |= (unsigned short)(exp_avg_sq[at1] << 8);
+        p1 = toFloat(param[at1]);
+        g1 = toFloat(grad[at1]);
+      }
+      m[j] = fromCodes(mc) * two(ms, ms);
+      root[j] = fromCodes(vc) * two(vs, vs);
+      const float2 next = split(updatePair(two(p0, p1), two(g0, g1) * scale_grad, m[j], root[j], c));
+      float2 a = split(m[j]), b = split(root[j]);
+      if (in0) param[at0] = fromFloat<P>(next.x);
+      else a.x = b.x = 0.0f;
+      if (in1) param[at1] = fromFloat<P>(next.y);
+      else a.y = b.y = 0.0f;
+      m_max = largest(largest(m_max, a.x), a.y);
+      v_max = largest(largest(v_max, b.x), b.y);
     }
     const BlockScale m_scale = blockScale(m_max), v_scale = blockScale(v_max);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int at = block * (int)kScaleBlock + j * 32 + lane;
-      if (at < count) {
-        exp_avg[at] = toCode(__fmul_rn(m[j], m_scale.inverse));
-        exp_avg_sq[at] = toCode(rootCode(root[j], v_scale.inverse));
+    for (int j = 0; j < 4; ++j) {
+      const int at0 = block * (int)kScaleBlock + 2 * j * 32 + lane, at1 = at0 + 32;
+      const unsigned short mc = toCodes(m[j] * two(m_scale.inverse, m_scale.inverse));
+      const unsigned short vc = toCodes(rootCodes(root[j], v_scale.inverse));
+      if (at0 < count) {
+        exp_avg[at0] = (unsigned char)mc;
+        exp_avg_sq[at0] = (unsigned char)vc;
+      }
+      if (at1 < count) {
+        exp_avg[at1] = (unsigned char)(mc >> 8);
+        exp_avg_sq[at1] = (unsigned char)(vc >> 8);
       }
     }
     if (lane == 0) {
@@ -285,27 +362,23 @@ __global__ void __launch_bounds__(kThreads) adamW8BitKernel(const __grid_constan
 }
 
 template <typename P, typename G>
-cudaError_t launchTable(const TensorTable &t, bool state_8bit, int chunks, double bytes, cudaStream_t stream) {
-  if (state_8bit) {
-    trace::Scope scope("adamW8BitKernel", stream, bytes);
-    adamW8BitKernel<P, G><<<chunks, kThreads, 0, stream>>>(t);
-  } else {
-    trace::Scope scope("adamWKernel", stream, bytes);
-    adamWKernel<P, G><<<chunks, kThreads, 0, stream>>>(t);
-  }
+cudaError_t launchTable(const TensorTable &t, bool state_8bit, int chunk, int chunks, double bytes, cudaStream_t stream) {
+  trace::Scope scope(state_8bit ? "adamW8BitKernel" : "adamWKernel", stream, bytes);
+  auto kernel = state_8bit ? adamW8BitKernel<P, G> : chunk == kChunk ? adamWKernel<P, G, kChunk> : adamWKernel<P, G, kSmallChunk>;
+  kernel<<<chunks, kThreads, 0, stream>>>(t);
   return cudaGetLastError();
 }
 
-cudaError_t dispatch(const AdamWProblem &p, const TensorTable &t, int chunks, double bytes, cudaStream_t stream) {
+cudaError_t dispatch(const AdamWProblem &p, const TensorTable &t, int chunk, int chunks, double bytes, cudaStream_t stream) {
   const bool float_grad = p.grad_dtype == MLUOP_DTYPE_FLOAT;
   switch (p.param_dtype) {
-    case MLUOP_DTYPE_FLOAT: return launchTable<float, float>(t, p.state_8bit, chunks, bytes, stream);
+    case MLUOP_DTYPE_FLOAT: return launchTable<float, float>(t, p.state_8bit, chunk, chunks, bytes, stream);
     case MLUOP_DTYPE_HALF:
-      return float_grad ? launchTable<__half, float>(t, p.state_8bit, chunks, bytes, stream)
-                        : launchTable<__half, __half>(t, p.state_8bit, chunks, bytes, stream);
+      return float_grad ? launchTable<__half, float>(t, p.state_8bit, chunk, chunks, bytes, stream)
+                        : launchTable<__half, __half>(t, p.state_8bit, chunk, chunks, bytes, stream);
     default:
-      return float_grad ? launchTable<__nv_bfloat16, float>(t, p.state_8bit, chunks, bytes, stream)
-                        : launchTable<__nv_bfloat16, __nv_bfloat16>(t, p.state_8bit, chunks, bytes, stream);
+      return float_grad ? launchTable<__nv_bfloat16, float>(t, p.state_8bit, chunk, chunks, bytes, stream)
+                        : launchTable<__nv_bfloat16, __nv_bfloat16>(t, p.state_8bit, chunk, chunks, bytes, stream);
   }
 }
 
@@ -326,6 +399,11 @@ cudaError_t launchMultiTensorAdamW(const AdamWProblem &p, cudaStream_t stream) {
   t.c.root_scale = (float)(1.0 / std::sqrt(1.0 - std::pow(p.beta2, (double)p.step)));
   const double element_bytes = 2.0 * mluop::getSizeOfDataType(p.param_dtype) +
                                (double)mluop::getSizeOfDataType(p.grad_dtype) + (p.state_8bit ? 4.0 : 16.0);
+  // Float states, fewer chunks than four blocks an SM: smaller ones.  Measured on 24 tensors of 500,000 elements together:
+  // 7.7 us against 14 us.
+  int64_t all = 0;
+  for (int64_t k = 0; k < p.tensor_num; ++k) all += (p.element_num[k] + kChunk - 1) / kChunk;
+  const int chunk = p.state_8bit ? kChunk8Bit : all >= 4 * p.sm_count ? kChunk : kSmallChunk;
   int64_t i = 0;
   while (i < p.tensor_num) {
     int64_t chunks = 0, elements = 0;
@@ -333,7 +411,7 @@ cudaError_t launchMultiTensorAdamW(const AdamWProblem &p, cudaStream_t stream) {
     for (; i < p.tensor_num && k < kMaxTensors; ++i) {
       const int64_t n = p.element_num[i];
       if (n == 0) continue;
-      const int64_t more = (n + kChunk - 1) / kChunk;
+      const int64_t more = (n + chunk - 1) / chunk;
       if (k > 0 && chunks + more > INT32_MAX) break;  // (one tensor of 2^40 elements has 2^28 chunks)
       t.first_chunk[k] = (int)chunks;
       t.n[k] = n;
@@ -350,7 +428,7 @@ cudaError_t launchMultiTensorAdamW(const AdamWProblem &p, cudaStream_t stream) {
     if (k == 0) break;
     t.first_chunk[k] = (int)chunks;
     t.tensors = k;
-    const cudaError_t err = dispatch(p, t, (int)chunks, element_bytes * elements, stream);
+    const cudaError_t err = dispatch(p, t, chunk, (int)chunks, element_bytes * elements, stream);
     if (err != cudaSuccess) return err;
   }
   return cudaSuccess;

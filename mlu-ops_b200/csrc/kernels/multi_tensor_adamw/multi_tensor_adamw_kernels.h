@@ -25,6 +25,7 @@ struct AdamWProblem {
   double lr, beta1, beta2, epsilon, weight_decay;
   int64_t step;
   const float *grad_scale, *schedule;
+  int sm_count;
 };
 
 cudaError_t launchMultiTensorAdamW(const AdamWProblem &p, cudaStream_t stream);

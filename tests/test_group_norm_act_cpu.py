@@ -86,8 +86,8 @@ BOTH = [{"dtype": I32}, {"dims": (16,)}, {"groups": 3}, {"groups": 0}, {"groups"
         {"w": None}, {"b": None}, {"w": (FLOAT, (15,))}, {"w": (BF16, (16,)), "b": (BF16, (16,))},
         {"w": (HALF, (16,))}, {"mean": (HALF, (2, 4))}, {"rstd": (FLOAT, (4, 2))}, {"mean": (FLOAT, (8,))},
         {"dims": (2, 5, 16), "ends": True}, {"dims": (7, 16), "ends": True, "null": ("ends",)},
-        {"null": ("x",)}, {"null": ("w",)}, {"null": ("b",)}, {"null": ("mean",)}, {"null": ("rstd",)}, {"null": ("ws",)},
-        {"short": 1}, {"shift": {"x": 1}}, {"shift": {"w": 2}}, {"shift": {"mean": 2}}]
+        {"null": ("x",)}, {"null": ("w",)}, {"null": ("b",)}, {"null": ("mean",)}, {"null": ("rstd",)},
+        {"null": ("ws",), "dims": (2, 70000, 16)}, {"short": 1, "dims": (2, 70000, 16)}, {"shift": {"x": 1}}, {"shift": {"w": 2}}, {"shift": {"mean": 2}}]
 FORWARD = [{"eps": 0.0}, {"eps": -1.0}, {"eps": float("nan")}, {"y": (FLOAT, (2, 5, 16))}, {"y": (HALF, (2, 16, 5))},
            {"null": ("y",)}, {"shift": {"y": 1}}]
 BACKWARD = [{"dy": (FLOAT, (2, 5, 16))}, {"dy": (HALF, (10, 16))}, {"dx": (HALF, (2, 5, 8))}, {"null": ("dy",)}, {"null": ("dx",)},
@@ -103,6 +103,12 @@ def test_forward_refuses(ops, handle, over):
 @pytest.mark.parametrize("over", BOTH + BACKWARD)
 def test_backward_refuses(ops, handle, over):
     assert Call(ops, handle, **over).backward() == ops.STATUS_BAD_PARAM
+
+
+def test_few_rows_need_no_workspace(ops, handle):
+    c = Call(ops, handle, null=("ws",))
+    assert c.workspace(False) == (ops.STATUS_SUCCESS, 0) and c.workspace(True) == (ops.STATUS_SUCCESS, 0)
+    assert c.forward() == ops.STATUS_EXECUTION_FAILED and c.backward() == ops.STATUS_EXECUTION_FAILED
 
 
 def test_null_handle_and_descriptors(ops, handle):
