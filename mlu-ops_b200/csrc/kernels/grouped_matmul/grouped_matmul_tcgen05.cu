@@ -7,7 +7,7 @@
 //
 // No operand is transposed in memory: the tensor cores read either order from
 // swizzled shared memory, and TMA brings 64 x 64 boxes of any of the three matrices
-// there as they lie.
+// there as they lie (64 x 128 where the rows are the result axis).
 //
 // The grid is persistent.  Every block works out from the group ends which unit (a
 // tile of a group's result; for the weight gradient: of a chunk of its rows) is whose
@@ -374,16 +374,21 @@ groupedTcgen05Kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
           const unsigned bar = CTAS == 2 ? mapToRank(smemAddr(&full[s]), 0) : smemAddr(&full[s]);
           const unsigned a_dst = ring_addr + s * Cfg::kStageBytes, b_dst = a_dst + Cfg::kABytes;
           const int k0 = kb * kBlockK;
+          if (kAMn) {
 #pragma unroll
-          for (int i = 0; i < kBlockRows / kBox; ++i) {
-            if (kWeight) loadBox2<CTAS>(a_dst + i * kBoxBytes, a_map, u.m0 + (int)rank * kBlockRows + i * kBox, u.row0 + k0, bar);
-            else loadBox2<CTAS>(a_dst + i * kBoxBytes, a_map, k0, u.row0 + (int)rank * kBlockRows + i * kBox, bar);
+            for (int i = 0; i < kBlockRows / kBox; ++i)
+              loadBox2<CTAS>(a_dst + i * kBoxBytes, a_map, u.m0 + (int)rank * kBlockRows + i * kBox, u.row0 + k0, bar);
+          } else {
+            loadBox2<CTAS>(a_dst, a_map, k0, u.row0 + (int)rank * kBlockRows, bar);
           }
+          if (kBMn) {
 #pragma unroll
-          for (int i = 0; i < Cfg::kBColumns / kBox; ++i) {
-            if (kWeight) loadBox2<CTAS>(b_dst + i * kBoxBytes, b_map, b0 + i * kBox, u.row0 + k0, bar);
-            else if (kBMn) loadBox3<CTAS>(b_dst + i * kBoxBytes, b_map, b0 + i * kBox, k0, u.group, bar);
-            else loadBox3<CTAS>(b_dst + i * kBoxBytes, b_map, k0, b0 + i * kBox, u.group, bar);
+            for (int i = 0; i < Cfg::kBColumns / kBox; ++i) {
+              if (kWeight) loadBox2<CTAS>(b_dst + i * kBoxBytes, b_map, b0 + i * kBox, u.row0 + k0, bar);
+              else loadBox3<CTAS>(b_dst + i * kBoxBytes, b_map, b0 + i * kBox, k0, u.group, bar);
+            }
+          } else {
+            loadBox3<CTAS>(b_dst, b_map, k0, b0, u.group, bar);
           }
         }
       }
@@ -536,12 +541,12 @@ EncodeTiled encodeTiled() {
 }
 
 // Tensor map of a dense matrix or stack of matrices with `columns` contiguous 16-bit values.
-bool encode(CUtensorMap *map, const void *base, bool bf16, int64_t columns, int64_t rows, int64_t depth) {
+bool encode(CUtensorMap *map, const void *base, bool bf16, int64_t columns, int64_t rows, int64_t depth, int box_rows) {
   const EncodeTiled fn = encodeTiled();
   if (!fn) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)columns, (cuuint64_t)rows, (cuuint64_t)depth};
   const cuuint64_t strides[2] = {(cuuint64_t)columns * 2, (cuuint64_t)columns * rows * 2};
-  const cuuint32_t box[3] = {kBox, kBox, 1}, steps[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {kBox, (cuuint32_t)box_rows, 1}, steps[3] = {1, 1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, depth > 0 ? 3 : 2,
             const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -659,13 +664,13 @@ cudaError_t launchTensorCores(const Problem &p, const void *a, const void *b, co
   }
   CUtensorMap map_a, map_b;
   if (p.mode != kBackwardWeight) {
-    if (!encode(&map_a, a, bf16, p.mode == kForward ? p.ci : p.co, p.rows, 0) ||
-        !encode(&map_b, b, bf16, p.co, p.ci, p.groups))
+    if (!encode(&map_a, a, bf16, p.mode == kForward ? p.ci : p.co, p.rows, 0, kBlockRows) ||
+        !encode(&map_b, b, bf16, p.co, p.ci, p.groups, p.mode == kForward ? kBox : tile.columns / tile.ctas))
       return cudaErrorInvalidValue;
     return p.mode == kForward ? launchMode<kForward>(p, tile, map_a, map_b, params, stream)
                               : launchMode<kBackwardInput>(p, tile, map_a, map_b, params, stream);
   }
-  if (!encode(&map_a, a, bf16, p.ci, p.rows, 0) || !encode(&map_b, b, bf16, p.co, p.rows, 0)) return cudaErrorInvalidValue;
+  if (!encode(&map_a, a, bf16, p.ci, p.rows, 0, kBox) || !encode(&map_b, b, bf16, p.co, p.rows, 0, kBox)) return cudaErrorInvalidValue;
   const WeightGradPlan plan = planWeightGrad(p, true);
   char *base = reinterpret_cast<char *>((reinterpret_cast<size_t>(workspace) + 255) / 256 * 256);
   CUtensorMap *maps = reinterpret_cast<CUtensorMap *>(base + plan.maps);
