@@ -102,6 +102,13 @@ __device__ __forceinline__ void arriveRemote(unsigned cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
 }
 
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool electOne() {
+  unsigned r;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+
 // TMA loads of one box; `bar` is an address in the cluster's window (CTAS = 2: the leading block's barrier).
 template <int CTAS>
 __device__ __forceinline__ void loadBox2(unsigned dst, const CUtensorMap *map, int x, int y, unsigned bar) {
@@ -407,44 +414,54 @@ groupedTcgen05Kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       // ---------------------------------------------------------- products
+      // The whole warp walks the units, so that addresses and descriptors are the same in all lanes and live in uniform
+      // registers; one elected lane issues.
       const unsigned idesc = (1u << 4) | ((unsigned)p.bf16 << 7) | ((unsigned)p.bf16 << 10) | ((kAMn ? 1u : 0u) << 15) |
                              ((kBMn ? 1u : 0u) << 16) | ((unsigned)(BN >> 3) << 17) |
                              ((unsigned)((kBlockRows * CTAS) >> 4) << 24);
       constexpr unsigned kAStep = (kAMn ? 16 * 128 : 32) >> 4, kBStep = (kBMn ? 16 * 128 : 32) >> 4;
-      unsigned it = 0, done = 0;
-      bool ok = true;
+      const unsigned long long a_desc = operandDesc(ring_addr, kAMn), b_desc = operandDesc(ring_addr + Cfg::kABytes, kBMn);
+      unsigned s = 0, parity = 0, done = 0;
+      bool ok = true, first = true;
       for (int unit = first_unit; unit < units && ok; unit += stride) {
         const Unit u = unitAt<MODE, CTAS, BN>(map, p, m_tiles, n_tiles, unit);
         if (u.k_blocks == 0) continue;
         const unsigned acc = done & 1u;
-        if (done >= 2 && !mbarWait(&sums_empty[acc], ((done >> 1) - 1u) & 1u, abort_flag, sink, kErrIssuer, p.wait_limit)) {
+        if (done >= 2 && !mbarWaitWarp(&sums_empty[acc], ((done >> 1) - 1u) & 1u, abort_flag, sink, kErrIssuer, p.wait_limit)) {
           ok = false;
           break;
         }
         tcFenceAfter();
         const unsigned d = tmem_base + acc * BN;
-        for (int kb = 0; kb < u.k_blocks; ++kb, ++it) {
-          const unsigned s = it % S;
-          if (!mbarWait(&full[s], (it / S) & 1u, abort_flag, sink, kErrIssuer, p.wait_limit)) {
+        for (int kb = 0; kb < u.k_blocks; ++kb) {
+          if (!mbarWaitWarp(&full[s], parity, abort_flag, sink, kErrIssuer, p.wait_limit)) {
             ok = false;
             break;
           }
           tcFenceAfter();
-          const unsigned a_addr = ring_addr + s * Cfg::kStageBytes;
-          const unsigned long long a = operandDesc(a_addr, kAMn), b = operandDesc(a_addr + Cfg::kABytes, kBMn);
+          if (electOne()) {
+            // only the start-address field (16-byte units) differs between stages and steps
+            const unsigned long long a = a_desc + (unsigned long long)(s * (Cfg::kStageBytes >> 4));
+            const unsigned long long b = b_desc + (unsigned long long)(s * (Cfg::kStageBytes >> 4));
 #pragma unroll
-          for (int j = 0; j < kBlockK / 16; ++j)
-            mma<CTAS>(d, a + (unsigned long long)(j * kAStep), b + (unsigned long long)(j * kBStep), idesc, kb > 0 || j > 0 ? 1u : 0u);
-          // (test hook: the first release of a block is withheld, so that the loads' wait for that stage runs out)
-          if (!(p.test_drop_release && it == 0)) commit<CTAS>(&empty[s]);
+            for (int j = 0; j < kBlockK / 16; ++j)
+              mma<CTAS>(d, a + (unsigned long long)(j * kAStep), b + (unsigned long long)(j * kBStep), idesc, kb > 0 || j > 0 ? 1u : 0u);
+            // (test hook: the first release of a block is withheld, so that the loads' wait for that stage runs out)
+            if (!(p.test_drop_release && first)) commit<CTAS>(&empty[s]);
+            if (kb + 1 == u.k_blocks) commit<CTAS>(&sums_full[acc]);
+          }
+          __syncwarp();
+          first = false;
+          if (++s == S) {
+            s = 0;
+            parity ^= 1u;
+          }
         }
-        if (!ok) break;
-        commit<CTAS>(&sums_full[acc]);
         ++done;
       }
-      if (*abort_flag) {
+      if (*abort_flag && electOne()) {
         // leaving early: MMAs may still be running; tensor memory must not be freed under them
         commit<CTAS>(&drain_bar);
         const long long t0 = clock64();
