@@ -354,29 +354,28 @@ groupedTcgen05Kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   const unsigned ring_addr = smemAddr(ring);
 
   if (warp == 0) {
-    if (lane == 0) {
-      // ---------------------------------------------------------- loads
-      unsigned it = 0;
-      bool ok = true;
-      int known_group = -1;
-      for (int unit = first_unit; unit < units && ok; unit += stride) {
-        const Unit u = unitAt<MODE, CTAS, BN>(map, p, m_tiles, n_tiles, unit);
-        if (kWeight && u.k_blocks > 0 && u.group != known_group) {
-          // the group's maps were written by the kernel before this one
-          known_group = u.group;
+    // ------------------------------------------------------------ loads (one elected lane issues)
+    unsigned s = 0, parity = 0, issued = 0;
+    bool ok = true;
+    int known_group = -1;
+    for (int unit = first_unit; unit < units && ok; unit += stride) {
+      const Unit u = unitAt<MODE, CTAS, BN>(map, p, m_tiles, n_tiles, unit);
+      if (kWeight && u.k_blocks > 0 && u.group != known_group) {
+        // the group's maps were written by the kernel before this one
+        known_group = u.group;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;\n" ::"l"(p.group_maps + 2 * u.group + i) : "memory");
+        for (int i = 0; i < 2; ++i)
+          asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;\n" ::"l"(p.group_maps + 2 * u.group + i) : "memory");
+      }
+      const CUtensorMap *a_map = kWeight ? p.group_maps + 2 * u.group : &map_a;
+      const CUtensorMap *b_map = kWeight ? p.group_maps + 2 * u.group + 1 : &map_b;
+      const int b0 = u.n0 + (int)rank * Cfg::kBColumns;
+      for (int kb = 0; kb < u.k_blocks; ++kb, ++issued) {
+        if (issued >= S && !mbarWaitWarp(&empty[s], parity ^ 1u, abort_flag, sink, kErrProducer, p.wait_limit)) {
+          ok = false;
+          break;
         }
-        const CUtensorMap *a_map = kWeight ? p.group_maps + 2 * u.group : &map_a;
-        const CUtensorMap *b_map = kWeight ? p.group_maps + 2 * u.group + 1 : &map_b;
-        const int b0 = u.n0 + (int)rank * Cfg::kBColumns;
-        for (int kb = 0; kb < u.k_blocks; ++kb, ++it) {
-          const unsigned s = it % S;
-          if (it >= S && !mbarWait(&empty[s], ((it / S) - 1u) & 1u, abort_flag, sink, kErrProducer, p.wait_limit)) {
-            ok = false;
-            break;
-          }
+        if (electOne()) {
           if (rank == 0) mbarArriveExpectTx(&full[s], CTAS * Cfg::kStageBytes);
           const unsigned bar = CTAS == 2 ? mapToRank(smemAddr(&full[s]), 0) : smemAddr(&full[s]);
           const unsigned a_dst = ring_addr + s * Cfg::kStageBytes, b_dst = a_dst + Cfg::kABytes;
@@ -398,18 +397,23 @@ groupedTcgen05Kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             loadBox3<CTAS>(b_dst, b_map, k0, b0, u.group, bar);
           }
         }
+        __syncwarp();
+        if (++s == S) {
+          s = 0;
+          parity ^= 1u;
+        }
       }
-      if (*abort_flag) {
-        // leaving early: see the copies in flight out (bounded); the other block's count on the leader's barriers
-        const long long t0 = clock64();
-        if (rank == 0) {
-          for (unsigned i = it > S ? it - S : 0; i < it; ++i) {
-            while (!mbarTryWait(&full[i % S], (i / S) & 1u) && clock64() - t0 <= 1000000) {
-            }
+    }
+    if (*abort_flag) {
+      // leaving early: see the copies in flight out (bounded); the other block's count on the leader's barriers
+      const long long t0 = clock64();
+      if (rank == 0) {
+        for (unsigned i = issued > S ? issued - S : 0; i < issued; ++i) {
+          while (!mbarTryWait(&full[i % S], (i / S) & 1u) && clock64() - t0 <= 1000000) {
           }
         }
-        while (clock64() - t0 <= 1000000) {
-        }
+      }
+      while (clock64() - t0 <= 1000000) {
       }
     }
     __syncwarp();
