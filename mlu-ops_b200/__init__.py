@@ -181,6 +181,7 @@ class Handle:
 
     def set_queue(self, stream):
         check("mluOpSetQueue", lib().mluOpSetQueue(self.ptr, _vp(stream)))
+        self.stream = stream
 
     def destroy(self):
         if self.ptr:
@@ -795,23 +796,27 @@ def _call_plan(handle, key, specs, query=None):
     return plan
 
 
-def _new(like, shape, dtype):
+def _new(handle, like, shape, dtype):
+    """A tensor that the handle's queue may use at once: where that is not the current stream, from the queue's own memory
+    pool, and kept until the current stream is done with it too."""
     if _guards is not None:
         return _guards.empty(shape, dtype, like.device)
-    return like.new_empty(shape, dtype=dtype)
-
-
-def _new_like(t):
     import torch
-    return torch.empty_like(t) if _guards is None else _guards.empty(t.shape, t.dtype, t.device)
+    if handle.device < 0 or torch._C._cuda_getCurrentRawStream(handle.device) == (handle.stream or 0):
+        return like.new_empty(shape, dtype=dtype)
+    current = torch.cuda.current_stream(handle.device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(handle.stream or 0, device=handle.device)):
+        t = like.new_empty(shape, dtype=dtype)
+    t.record_stream(current)
+    return t
 
 
-def _workspace(like, nbytes):
+def _workspace(handle, like, nbytes):
     """(tensor, address) of a workspace; (None, None) if none is needed."""
     import torch
     if nbytes == 0:
         return None, None
-    t = _new(like, (nbytes,), torch.uint8)
+    t = _new(handle, like, (nbytes,), torch.uint8)
     return t, t.data_ptr()
 
 
@@ -845,8 +850,8 @@ def group_norm_act_forward(handle, input, weight, bias, num_groups, epsilon=1e-5
     num_groups = int(num_groups)
     stats = ((input.shape[0] if sample_ends is None else sample_ends.shape[0]), num_groups)
     if out is None:
-        out = _new_like(input)
-    mean, rstd = _new(input, stats, torch.float32), _new(input, stats, torch.float32)
+        out = _new(handle, input, input.shape, input.dtype)
+    mean, rstd = _new(handle, input, stats, torch.float32), _new(handle, input, stats, torch.float32)
     p_y = _address(handle, "out", out)
     specs = lambda: [_spec(t) for t in (input, weight, bias, sample_ends, out)] + [(torch.float32, stats)]  # noqa: E731
     plan = _call_plan(handle, ("norm", num_groups, input.shape, input.dtype, out.shape, out.dtype, _spec(weight),
@@ -855,7 +860,7 @@ def group_norm_act_forward(handle, input, weight, bias, num_groups, epsilon=1e-5
                                                lib().mluOpGetGroupNormActForwardWorkspaceSize(
                                                    handle.ptr, plan.d[0], plan.d[3], num_groups, ctypes.byref(size))))
     d_x, d_w, d_b, d_e, d_y, d_m = plan.d
-    workspace, p_s = _workspace(input, plan.workspace)
+    workspace, p_s = _workspace(handle, input, plan.workspace)
     check("mluOpGroupNormActForward",
           lib().mluOpGroupNormActForward(handle.ptr, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, num_groups, epsilon, act,
                                          p_s, plan.workspace, d_y, p_y, d_m, mean.data_ptr(), d_m, rstd.data_ptr()))
@@ -880,12 +885,12 @@ def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd
     p_m, p_r = _address(handle, "mean", mean), _address(handle, "rstd", rstd)
     num_groups = int(num_groups)
     if out is None:
-        out = _new_like(input)
+        out = _new(handle, input, input.shape, input.dtype)
     p_o = _address(handle, "out", out)
     weight_grad = bias_grad = p_wg = p_bg = None
     if affine_grad:
-        weight_grad = _new(input, input.shape[-1:], affine_grad_dtype or torch.float32)
-        bias_grad = _new(input, input.shape[-1:], affine_grad_dtype or torch.float32)
+        weight_grad = _new(handle, input, input.shape[-1:], affine_grad_dtype or torch.float32)
+        bias_grad = _new(handle, input, input.shape[-1:], affine_grad_dtype or torch.float32)
         p_wg, p_bg = weight_grad.data_ptr(), bias_grad.data_ptr()
     tensors = (output_grad, input, weight, bias, sample_ends, mean, rstd, out, weight_grad, bias_grad)
     plan = _call_plan(handle, ("norm_grad", num_groups) + tuple([_spec(t) for t in tensors]),
@@ -894,7 +899,7 @@ def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd
                                                lib().mluOpGetGroupNormActBackwardWorkspaceSize(
                                                    handle.ptr, plan.d[1], plan.d[4], num_groups, ctypes.byref(size))))
     d_g, d_x, d_w, d_b, d_e, d_m, d_r, d_o, d_wg, d_bg = plan.d
-    workspace, p_s = _workspace(input, plan.workspace)
+    workspace, p_s = _workspace(handle, input, plan.workspace)
     check("mluOpGroupNormActBackward",
           lib().mluOpGroupNormActBackward(handle.ptr, d_g, p_g, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, d_m, p_m, d_r,
                                           p_r, num_groups, act, p_s, plan.workspace, d_o, p_o, d_wg, p_wg, d_bg,
@@ -1003,7 +1008,7 @@ def grouped_matmul_forward(handle, input, weight, group_ends, out=None):
     p_x, p_w, p_e = (_address(handle, "input", input), _address(handle, "weight", weight),
                      _address(handle, "group_ends", group_ends))
     if out is None:
-        out = _new(input, (input.shape[0], weight.shape[-1]), input.dtype)
+        out = _new(handle, input, (input.shape[0], weight.shape[-1]), input.dtype)
     p_y = _address(handle, "out", out)
     tensors = (input, weight, group_ends, out)
     plan = _call_plan(handle, ("product", input.shape, input.dtype, weight.shape, weight.dtype, group_ends.shape,
@@ -1020,7 +1025,7 @@ def grouped_matmul_backward_input(handle, output_grad, weight, group_ends, out=N
     p_g, p_w, p_e = (_address(handle, "output_grad", output_grad), _address(handle, "weight", weight),
                      _address(handle, "group_ends", group_ends))
     if out is None:
-        out = _new(output_grad, (output_grad.shape[0], weight.shape[-2]), output_grad.dtype)
+        out = _new(handle, output_grad, (output_grad.shape[0], weight.shape[-2]), output_grad.dtype)
     p_x = _address(handle, "out", out)
     tensors = (output_grad, weight, group_ends, out)
     plan = _call_plan(handle, ("product", output_grad.shape, output_grad.dtype, weight.shape, weight.dtype,
@@ -1038,7 +1043,7 @@ def grouped_matmul_backward_weight(handle, input, output_grad, group_ends, dtype
     p_x, p_g, p_e = (_address(handle, "input", input), _address(handle, "output_grad", output_grad),
                      _address(handle, "group_ends", group_ends))
     if out is None:
-        out = _new(input, (group_ends.shape[0], input.shape[-1], output_grad.shape[-1]), dtype or input.dtype)
+        out = _new(handle, input, (group_ends.shape[0], input.shape[-1], output_grad.shape[-1]), dtype or input.dtype)
     p_w = _address(handle, "out", out)
     tensors = (input, output_grad, group_ends, out)
     plan = _call_plan(handle, ("product_weight", input.shape, input.dtype, output_grad.shape, output_grad.dtype,
@@ -1048,7 +1053,7 @@ def grouped_matmul_backward_weight(handle, input, output_grad, group_ends, dtype
                                                lib().mluOpGetGroupedMatMulBackwardWeightWorkspaceSize(
                                                    handle.ptr, plan.d[0], plan.d[1], plan.d[3], ctypes.byref(size))))
     d_x, d_g, d_e, d_w = plan.d
-    workspace, p_s = _workspace(input, plan.workspace)
+    workspace, p_s = _workspace(handle, input, plan.workspace)
     check("mluOpGroupedMatMulBackwardWeight",
           lib().mluOpGroupedMatMulBackwardWeight(handle.ptr, d_x, p_x, d_g, p_g, d_e, p_e, p_s, plan.workspace, d_w,
                                                  p_w))

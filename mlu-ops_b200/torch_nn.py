@@ -1,0 +1,227 @@
+"""PyTorch modules over the C ABI for what stands between and behind the convolutions of a
+training step: group norm with an activation, products grouped by row blocks, the AdamW step.
+
+    x = SubMConv3d(16, 64, 3)(x)
+    x = GroupNormAct(8, 64, activation="relu")(x)          # per sample of the sparse tensor
+    y = GroupedLinear(num_groups, 64, 128)(rows, ends)      # one matrix for each block of rows
+    AdamW(model.parameters(), lr=1e-3, state_bits=8).step()
+
+Every tensor stays on the GPU and nothing is read back.  There is no CPU path.
+"""
+import math
+import sys
+
+import torch
+from torch import nn
+
+from .torch_sparse import SparseConvTensor, _handle
+
+ops = sys.modules[__package__]
+
+
+class _GroupedMatMul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input, weight, group_ends):
+        input, weight = input.contiguous(), weight.contiguous()
+        ctx.save_for_backward(input, weight, group_ends)
+        return ops.grouped_matmul_forward(_handle(input.device), input, weight, group_ends)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        input, weight, group_ends = ctx.saved_tensors
+        grad = grad.contiguous()
+        h = _handle(input.device)
+        grad_input = grad_weight = None
+        if ctx.needs_input_grad[0]:
+            grad_input = ops.grouped_matmul_backward_input(h, grad, weight, group_ends)
+        if ctx.needs_input_grad[1]:
+            grad_weight = ops.grouped_matmul_backward_weight(h, input, grad, group_ends)
+        return grad_input, grad_weight, None
+
+
+def grouped_matmul(input, weight, group_ends):
+    """output[r] = input[r] @ weight[g] for the rows r of group g, differentiable in input and weight
+    (mluOpGroupedMatMul*).  input [rows,Ci], weight [G,Ci,Co]; group_ends int32 [G] on the device: group
+    g's rows end there and the next group's begin.  Rows behind the last end give zeros and get zeros."""
+    return _GroupedMatMul.apply(input, weight, group_ends)
+
+
+class GroupedLinear(nn.Module):
+    """A linear layer with a matrix of its own for each block of rows (experts, classes, levels)."""
+
+    def __init__(self, num_groups, in_channels, out_channels, dtype=torch.float32):
+        super().__init__()
+        self.weight = nn.Parameter(torch.empty(int(num_groups), int(in_channels), int(out_channels), dtype=dtype))
+        bound = 1.0 / math.sqrt(in_channels)
+        nn.init.uniform_(self.weight, -bound, bound)
+
+    def forward(self, input, group_ends):
+        return grouped_matmul(input, self.weight, group_ends)
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input, weight, bias, num_groups, epsilon, activation, sample_ends):
+        input = input.contiguous()
+        out, mean, rstd = ops.group_norm_act_forward(_handle(input.device), input, weight, bias, num_groups, epsilon,
+                                                     activation, sample_ends)
+        ctx.save_for_backward(input, weight, bias, mean, rstd, sample_ends)
+        ctx.num_groups, ctx.activation = num_groups, activation
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        input, weight, bias, mean, rstd, sample_ends = ctx.saved_tensors
+        affine = weight is not None and (ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        grad_input, grad_weight, grad_bias = ops.group_norm_act_backward(
+            _handle(input.device), grad.contiguous(), input, weight, bias, mean, rstd, ctx.num_groups, ctx.activation,
+            sample_ends, affine_grad=affine, affine_grad_dtype=weight.dtype if affine else None)
+        needs = ctx.needs_input_grad
+        return (grad_input if needs[0] else None, grad_weight if needs[1] else None, grad_bias if needs[2] else None, None,
+                None, None, None)
+
+
+def group_norm_act(input, num_groups, weight=None, bias=None, epsilon=1e-5, activation="none", sample_ends=None):
+    """Group norm over channels-last values with an activation ("none", "relu", "silu"), differentiable
+    in input, weight and bias (mluOpGroupNormAct*).  input [N, ..., C], each index of the first dimension a
+    sample; or [rows, C] with sample_ends int32 [N] on the device, where each sample's rows end."""
+    return _GroupNormAct.apply(input, weight, bias, num_groups, epsilon, activation, sample_ends)
+
+
+class GroupNormAct(nn.Module):
+    """group_norm_act as a module, for tensors [N, ..., C] and for a SparseConvTensor, whose samples are
+    normalised one by one (its rows in ascending order of the batch index)."""
+
+    def __init__(self, num_groups, num_channels, epsilon=1e-5, affine=True, activation="none", dtype=torch.float32):
+        super().__init__()
+        self.num_groups, self.epsilon, self.activation = int(num_groups), float(epsilon), activation
+        self.weight = nn.Parameter(torch.ones(num_channels, dtype=dtype)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels, dtype=dtype)) if affine else None
+
+    def forward(self, x):
+        if not isinstance(x, SparseConvTensor):
+            return group_norm_act(x, self.num_groups, self.weight, self.bias, self.epsilon, self.activation)
+        ends = x.sample_ends()
+        out = SparseConvTensor(group_norm_act(x.features, self.num_groups, self.weight, self.bias, self.epsilon,
+                                              self.activation, ends),
+                               x.indices, x.spatial_shape, x.batch_size, x.indice_dict)
+        out._sample_ends = ends
+        return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with one launch for up to 480 tensors (mluOpMultiTensorAdamW).
+
+    state_bits: 32, or 8 for states of one byte an element and one scale for 256 elements (first moment
+    and square root of the second in e4m3).  Parameters are dense CUDA tensors in float32, float16 or
+    bfloat16; states are held in float or 8 bits whatever the parameter's type.  capturable=True keeps the
+    step count and the learning rate of each parameter group on the device, so that a captured step can be
+    replayed (lr may then be a CUDA tensor; one step count for the whole group).  step(grad_scale=t)
+    multiplies every gradient by the float32 CUDA tensor t of one element.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits is 8 or 32")
+        if not torch.is_tensor(lr) and not lr >= 0.0:
+            raise ValueError("lr must not be negative")
+        if torch.is_tensor(lr) and not capturable:
+            raise ValueError("a tensor as lr needs capturable=True")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
+            raise ValueError("0 <= beta < 1, eps >= 0 and weight_decay >= 0 are required")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.capturable = state_bits, bool(capturable)
+        self._plans = {}      # the tensors of each bucket, checked and laid out for the call
+        self._schedules = {}  # capturable: per group (step count, {lr, 1 - beta1^step, 1 - beta2^step})
+
+    def _new_state(self, p):
+        if self.state_bits == 32:
+            zeros = [torch.zeros(p.numel(), dtype=torch.float32, device=p.device) for _ in range(2)]
+            return {"step": 0, "exp_avg": zeros[0].view(p.shape), "exp_avg_sq": zeros[1].view(p.shape)}
+        blocks = -(-p.numel() // ops.SCALE_BLOCK)
+        state = {"step": 0}
+        for key in ("exp_avg", "exp_avg_sq"):
+            state[key] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+            state[key + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        return state
+
+    def _bucket(self, key, params):
+        """The plan for these parameters, built anew where a parameter or state lies elsewhere than before."""
+        states = [self.state[p] for p in params]
+        keys = ["exp_avg", "exp_avg_sq"] + (["exp_avg_scale", "exp_avg_sq_scale"] if self.state_bits == 8 else [])
+        tensors = [params] + [[s[k] for s in states] for k in keys]
+        at = [list(map(torch.Tensor.data_ptr, v)) for v in tensors]
+        known = self._plans.get(key)
+        if known is None or known[0] != at:
+            known = self._plans[key] = (at, ops.MultiTensorAdamW(*tensors))
+        return known[1]
+
+    def _schedule(self, index, group, device):
+        """Capturable: counts the group's step on the device and returns its schedule tensor."""
+        if index not in self._schedules:
+            self._schedules[index] = (torch.zeros((), dtype=torch.float64, device=device),
+                                      torch.tensor([1.0, *group["betas"]], dtype=torch.float64, device=device))
+        count, base = self._schedules[index]
+        count += 1
+        powers = 1.0 - base ** count
+        lr = group["lr"]
+        powers[0] = lr if torch.is_tensor(lr) else float(lr)
+        return powers.to(torch.float32)
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for index, group in enumerate(self.param_groups):
+            buckets = {}
+            for i, p in enumerate(group["params"]):
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise ValueError("sparse gradients are not supported")
+                state = self.state[p]
+                if not state:
+                    state.update(self._new_state(p))
+                state["step"] += 1
+                count = 0 if self.capturable else state["step"]
+                buckets.setdefault((p.device, p.dtype, p.grad.dtype, count), []).append((i, p))
+            schedules = {}
+            for (device, dtype, grad_dtype, count), members in buckets.items():
+                plan = self._bucket((index, device, dtype, grad_dtype, tuple(i for i, _ in members)), [p for _, p in members])
+                more = {}
+                if self.capturable:
+                    if device not in schedules:
+                        if schedules:
+                            raise ValueError("capturable: the parameters of a group lie on one device")
+                        schedules[device] = self._schedule(index, group, device)
+                    more["schedule"] = schedules[device]
+                lr = 0.0 if self.capturable else float(group["lr"])
+                plan.step(_handle(device), [p.grad.contiguous() for _, p in members], lr, group["betas"], group["eps"],
+                          group["weight_decay"], max(count, 1), grad_scale=grad_scale, **more)
+        return loss
+
+    def state_dict(self):
+        out = super().state_dict()
+        out["schedules"] = {i: (c.clone(), b.clone()) for i, (c, b) in self._schedules.items()}
+        return out
+
+    def load_state_dict(self, state_dict):
+        """As Optimizer.load_state_dict, with the states in the types they were saved in (the base class would cast
+        them to the parameters')."""
+        state_dict = dict(state_dict)
+        schedules = state_dict.pop("schedules", {})
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, params):
+            for key, value in state_dict["state"].get(i, {}).items():
+                self.state[p][key] = value.detach().clone().to(p.device) if torch.is_tensor(value) else value
+        self._schedules = {i: tuple(t.detach().clone() for t in pair) for i, pair in schedules.items()}
+        for i, pair in self._schedules.items():
+            device = self.param_groups[i]["params"][0].device
+            self._schedules[i] = tuple(t.to(device) for t in pair)
+        self._plans = {}

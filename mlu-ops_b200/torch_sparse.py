@@ -21,6 +21,7 @@ layout), float16 or float32 like the features.  There is no CPU path.
 """
 import math
 import sys
+import threading
 
 import torch
 from torch import nn
@@ -31,10 +32,12 @@ _handles = {}
 
 
 def _handle(device):
-    """One library handle per device, bound to the stream that is current at each call."""
-    key = device.index if device.index is not None else torch.cuda.current_device()
+    """One library handle per device and thread (autograd runs backward passes in threads of its own),
+    bound to the stream that is current at each call."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    key = (index, threading.get_ident())
     if key not in _handles:
-        with torch.cuda.device(key):
+        with torch.cuda.device(index):
             _handles[key] = ops.Handle(0)
     h = _handles[key]
     h.set_queue(torch.cuda.current_stream(device).cuda_stream)
@@ -82,6 +85,18 @@ class SparseConvTensor:
         self.spatial_shape = [int(v) for v in spatial_shape]
         self.batch_size = int(batch_size)
         self.indice_dict = {} if indice_dict is None else indice_dict
+
+    def sample_ends(self):
+        """int32 [batch_size] on the device: where each sample's rows end, for operators that work sample by sample.  The
+        rows must lie in ascending order of the batch index (one host read at the first call; kept with the tensor)."""
+        ends = getattr(self, "_sample_ends", None)
+        if ends is None:
+            batch = self.indices[:, 0].contiguous()
+            if batch.numel() and bool((batch[1:] < batch[:-1]).any() | (batch[0] < 0) | (batch[-1] >= self.batch_size)):
+                raise ValueError("the rows are not in ascending order of their batch index")
+            ends = torch.searchsorted(batch, torch.arange(1, self.batch_size + 1, dtype=torch.int32, device=batch.device))
+            self._sample_ends = ends = ends.to(torch.int32)
+        return ends
 
     def dense(self):
         """[batch, C, D, H, W] with zeros where no voxel is active."""
