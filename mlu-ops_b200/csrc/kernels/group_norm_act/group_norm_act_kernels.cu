@@ -51,9 +51,12 @@ struct Lanes {
   int columns, row_threads;
 };
 
-// A thread's sums (a, b) of each of its channels, added over the block's row threads in a fixed order; store(channel, sum)
-// is called once for each of the block's channels.  The values lie side by side in `scratch`, so that lanes read and
-// write neighbouring words, and are added in two steps, `parts` threads to a channel first.
+// Bytes of scratch that joinRowThreads needs.
+__host__ __device__ constexpr size_t joinBytes(int vec, int threads) { return (size_t)threads * (vec > 2 ? vec : 2) * sizeof(float2); }
+
+// A thread's sums (a, b) of each of its channels, added over the block's row threads in double and in a fixed order;
+// store(channel, sums) is called once for each of the block's channels.  The values lie side by side in `scratch`, so
+// that lanes read and write neighbouring words, and are added in two steps, `parts` threads to a channel first.
 template <int VEC, int THREADS, typename F>
 __device__ __forceinline__ void joinRowThreads(const Two (&a)[(VEC + 1) / 2], const Two (&b)[(VEC + 1) / 2], Lanes l,
                                                float2 *scratch, F store) {
@@ -70,9 +73,9 @@ __device__ __forceinline__ void joinRowThreads(const Two (&a)[(VEC + 1) / 2], co
   const int items = VEC * l.columns;  // (j, column), column fastest
   int parts = THREADS / items;
   parts = parts < 1 ? 1 : (parts > l.row_threads ? l.row_threads : parts);
-  int rows = l.row_threads;
+  double2 *joined = reinterpret_cast<double2 *>(scratch);  // (j, part, column) after the first step
   if (parts > 1) {
-    float2 s = make_float2(0.0f, 0.0f);
+    double2 s = make_double2(0.0, 0.0);
     const int column = tid % l.columns, part = tid / l.columns % parts, j = tid / (l.columns * parts);
     if (j < VEC) {
       for (int row = part; row < l.row_threads; row += parts) {
@@ -82,17 +85,24 @@ __device__ __forceinline__ void joinRowThreads(const Two (&a)[(VEC + 1) / 2], co
       }
     }
     __syncthreads();
-    if (j < VEC) scratch[tid] = s;
+    if (j < VEC) joined[tid] = s;
     __syncthreads();
-    rows = parts;
   }
   for (int item = tid; item < items; item += THREADS) {
     const int column = item % l.columns, j = item / l.columns;
-    float2 s = make_float2(0.0f, 0.0f);
-    for (int row = 0; row < rows; ++row) {
-      const float2 v = scratch[(j * rows + row) * l.columns + column];
-      s.x += v.x;
-      s.y += v.y;
+    double2 s = make_double2(0.0, 0.0);
+    if (parts > 1) {
+      for (int part = 0; part < parts; ++part) {
+        const double2 v = joined[(j * parts + part) * l.columns + column];
+        s.x += v.x;
+        s.y += v.y;
+      }
+    } else {
+      for (int row = 0; row < l.row_threads; ++row) {
+        const float2 v = scratch[j * used + row * l.columns + column];
+        s.x += v.x;
+        s.y += v.y;
+      }
     }
     store(column * VEC + j, s);
   }
@@ -120,7 +130,7 @@ __device__ __forceinline__ void forSamples(const Rows &r, int64_t begin, int64_t
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, 4)
 statisticsKernel(const T *x, Rows r, int channels, Lanes l, float2 *partial) {
-  extern __shared__ float2 scratch[];
+  extern __shared__ __align__(16) float2 scratch[];
   constexpr int kPairs = (VEC + 1) / 2;
   const int column = threadIdx.x % l.columns, row = threadIdx.x / l.columns;
   const int first0 = blockIdx.y * l.columns * VEC, first = first0 + column * VEC;
@@ -160,13 +170,12 @@ statisticsKernel(const T *x, Rows r, int channels, Lanes l, float2 *partial) {
         add(v);
       }
     }
-    const float n = (float)(stop - at);
+    const double n = (double)(stop - at);
     float2 *out = partial + (blockIdx.x + sample) * channels + first0;
-    joinRowThreads<VEC, kThreads>(a, b, l, scratch, [&](int c, float2 s) {
+    joinRowThreads<VEC, kThreads>(a, b, l, scratch, [&](int c, double2 s) {
       if (first0 + c >= channels) return;
-      const float k = toFloat(x[at * channels + first0 + c]);
-      const float off = s.x / n, squares = s.y - s.x * off;
-      out[c] = make_float2(k + off, squares < 0.0f ? 0.0f : squares);  // (NaN stays)
+      const double off = s.x / n, squares = s.y - s.x * off;
+      out[c] = make_float2((float)(toFloat(x[at * channels + first0 + c]) + off), squares < 0.0 ? 0.0f : (float)squares);
     });
   }, [](int64_t) {});
 }
@@ -290,7 +299,7 @@ template <typename T, int VEC, int ACT, bool UNIFORM>
 __global__ void __launch_bounds__(kThreads, 3)
 gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bool float_affine, const float *mean,
                const float *rstd, Rows r, int channels, int groups, Lanes l, float2 *partial) {
-  extern __shared__ float2 scratch[];
+  extern __shared__ __align__(16) float2 scratch[];
   constexpr int kPairs = (VEC + 1) / 2;
   const int column = threadIdx.x % l.columns, row = threadIdx.x / l.columns;
   const int first0 = blockIdx.y * l.columns * VEC, first = first0 + column * VEC;
@@ -336,8 +345,8 @@ gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bo
       }
     }
     float2 *out = partial + (blockIdx.x + sample) * channels + first0;
-    joinRowThreads<VEC, kThreads>(a, b, l, scratch, [&](int c, float2 s) {
-      if (first0 + c < channels) out[c] = s;
+    joinRowThreads<VEC, kThreads>(a, b, l, scratch, [&](int c, double2 s) {
+      if (first0 + c < channels) out[c] = make_float2((float)s.x, (float)s.y);
     });
   }, [](int64_t) {});
 }
@@ -473,9 +482,11 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
             Rows r, int channels, int groups, Lanes l, float epsilon, T *out, void *weight_grad, void *bias_grad,
             bool float_affine_grad) {
   constexpr int kPairs = (VEC + 1) / 2, kGroups = UNIFORM ? 1 : kPairs;
-  extern __shared__ float2 scratch[];  // [kSmallThreads * VEC] | the slice's channels | its groups
+  // joinRowThreads' scratch | the slice's channels (two doubles each) | its groups (two floats)
+  extern __shared__ __align__(16) float2 scratch[];
   const int slice = l.columns * VEC, group_channels = channels / groups, slice_groups = slice / group_channels;
-  float2 *sums = scratch + kSmallThreads * VEC, *stats = sums + slice;
+  double2 *sums = reinterpret_cast<double2 *>(scratch + joinBytes(VEC, kSmallThreads) / sizeof(float2));
+  float2 *stats = reinterpret_cast<float2 *>(sums + slice);
   const int tid = threadIdx.x, row = tid / l.columns;
   const int first0 = blockIdx.x * slice, own = tid % l.columns * VEC, first = first0 + own;
   const int group0 = first0 / group_channels;
@@ -522,7 +533,7 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
         }
       }
     }
-    joinRowThreads<VEC, kSmallThreads>(a, b, l, scratch, [&](int ch, float2 v) { sums[ch] = v; });
+    joinRowThreads<VEC, kSmallThreads>(a, b, l, scratch, [&](int ch, double2 v) { sums[ch] = v; });
     __syncthreads();
     if (BACKWARD) {
       if (tid < slice) {  // (slice <= kSmallThreads)
@@ -534,15 +545,15 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
       double u = 0.0, w = 0.0, ref = 0.0;
       for (int i = 0; i < group_channels; ++i) {
         const int ch = q * group_channels + i;
-        const float2 v = sums[ch];
+        const double2 v = sums[ch];
         if (BACKWARD) {
           const double gamma = weight ? (double)loadAffine<T>(weight, float_affine, first0 + ch) : 1.0;
           u += gamma * v.x;
           w += gamma * v.y;
         } else if (rows > 0) {  // (sum, squares) about the channel's first value
-          const double off = (double)v.x / rows, m = (double)toFloat(x[begin * channels + first0 + ch]) + off;
+          const double off = v.x / rows, m = (double)toFloat(x[begin * channels + first0 + ch]) + off;
           if (i == 0) ref = m;
-          const double squares = (double)v.y - (double)v.x * off;
+          const double squares = v.y - v.x * off;
           u += m - ref;
           w += (squares < 0.0 ? 0.0 : squares) + rows * (m - ref) * (m - ref);  // (NaN stays)
         }
@@ -654,7 +665,7 @@ cudaError_t launchSlices(const NormProblem &p, int columns, const void *output_g
                          cudaStream_t stream) {
   const Lanes l{columns, kSmallThreads / columns};
   const int slice = columns * VEC;
-  const size_t smem = ((size_t)kSmallThreads * VEC + slice + slice / (p.channels / p.groups)) * sizeof(float2);
+  const size_t smem = joinBytes(VEC, kSmallThreads) + slice * sizeof(double2) + slice / (p.channels / p.groups) * sizeof(float2);
   const dim3 grid((unsigned)(p.channels / slice), BACKWARD ? 1u : (unsigned)p.samples);
   trace::Scope scope(BACKWARD ? "groupNormSliceKernel:backward" : "groupNormSliceKernel:forward", stream,
                      (BACKWARD ? 3 : 2) * rowBytes(p));
@@ -678,7 +689,7 @@ cudaError_t forward(const NormProblem &p, const NormPlan &plan, const void *inpu
   const Rows r = rowsOf(p, plan);
   const Lanes l{plan.column_threads, plan.row_threads};
   const dim3 grid((unsigned)plan.blocks, (unsigned)plan.column_tiles);
-  const size_t smem = (size_t)kThreads * VEC * sizeof(float2);
+  const size_t smem = joinBytes(VEC, kThreads);
   {
     trace::Scope scope("groupNormStatisticsKernel", stream, rowBytes(p));
     statisticsKernel<T, VEC><<<grid, kThreads, smem, stream>>>(x, r, p.channels, l, partial);
@@ -712,7 +723,7 @@ cudaError_t backward(const NormProblem &p, const NormPlan &plan, const void *out
   const Rows r = rowsOf(p, plan);
   const Lanes l{plan.column_threads, plan.row_threads};
   const dim3 grid((unsigned)plan.blocks, (unsigned)plan.column_tiles);
-  const size_t smem = (size_t)kThreads * VEC * sizeof(float2);
+  const size_t smem = joinBytes(VEC, kThreads);
   {
     trace::Scope scope("groupNormGradSumsKernel", stream, 2 * rowBytes(p));
     gradSumsKernel<T, VEC, ACT, UNIFORM><<<grid, kThreads, smem, stream>>>(dy, x, weight, bias, p.float_affine, mean, rstd,

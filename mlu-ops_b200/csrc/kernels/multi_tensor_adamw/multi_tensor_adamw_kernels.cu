@@ -12,14 +12,15 @@
 // carries them.  Tensors are cut into chunks of 1024 to 4096 elements, a block each; a
 // block finds its tensor by bisection of the chunk counts.
 //
-// Float states: the roundings are those of the formula evaluated step by step.
+// The moments and the root are rounded as the formula evaluated step by step is, on
+// every path: a last bit that differs can tip an 8-bit code, which is 2^-4 of the
+// element at the next step.
 // 8-bit states: with 10 bytes an element the arithmetic is what has to be short.  It
-// runs on pairs of floats, with fused multiply-adds, and with the approximate square
-// root and reciprocal (2^-22 of the value; the states are rounded to 2^-4 of it
-// afterwards): 34 instructions an element.  Correctly rounded single operations took
-// 296 us for 10^8 bfloat16 elements, this form 177 us (1.0 GB: 5.7 TB/s).  One block
-// of 256 a warp and five blocks of threads an SM; two or four blocks a warp, their
-// loads ahead of their use, took 189 and 250 us.
+// runs on pairs of floats, and the change of the parameter, which no code depends on,
+// takes the approximate reciprocal (2^-22 of it).  Single operations and a correctly
+// rounded quotient took 296 us for 10^8 bfloat16 elements, this form 206 us (1.0 GB).
+// One block of 256 a warp and five blocks of threads an SM; two or four blocks a warp,
+// their loads ahead of their use, were slower by 4 and 35 %.
 //
 // 8-bit states: blocks of 256 consecutive elements share a float scale, one warp
 // takes one block (8 elements a lane), its largest magnitude by one warp reduction.
@@ -214,11 +215,9 @@ struct Pairs {
 };
 // Two elements: m and root (sqrt(v)) are updated in place.  Returns the new parameters.
 __device__ __forceinline__ Two updatePair(Two p, Two g, Two &m, Two &root, const Pairs &c) {
-  m = fma(g, c.one_minus_beta1, m * c.beta1);
-  float2 r = split(fma(g * g, c.one_minus_beta2, (root * root) * c.beta2));
-  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(r.x));
-  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(r.y));
-  root = two(r.x, r.y);
+  m = m * c.beta1 + g * c.one_minus_beta1;
+  const float2 r = split((root * root) * c.beta2 + (g * g) * c.one_minus_beta2);
+  root = two(__fsqrt_rn(r.x), __fsqrt_rn(r.y));
   float2 d = split(fma(root, c.root_scale, c.epsilon));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.x));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.y));
