@@ -1,5 +1,8 @@
-// Two floats in a register pair: one instruction of sm_100a works on both, each rounded as
-// the single operation is.
+// Two floats in a register pair: one instruction of sm_100a works on both.
+//
+// a * b + c written with the operators may become one fused multiply-add.  Where the
+// product has to be rounded by itself, addRounded adds: a multiply-add by a `one` that
+// the assembler cannot see to be 1.
 #ifndef MLUOP_B200_CORE_PAIR_CUH_
 #define MLUOP_B200_CORE_PAIR_CUH_
 
@@ -30,6 +33,11 @@ __device__ __forceinline__ Two operator+(Two a, Two b) {
 __device__ __forceinline__ Two operator*(Two a, Two b) {
   Two r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two addRounded(Two a, Two b, float one) {
+  Two r;
+  asm("{\n.reg .b64 o;\nmov.b64 o, {%3, %3};\nfma.rn.f32x2 %0, %1, o, %2;\n}" : "=l"(r.v) : "l"(a.v), "l"(b.v), "f"(one));
   return r;
 }
 __device__ __forceinline__ Two fma(Two a, Two b, Two c) {

@@ -14,6 +14,7 @@ namespace group_norm_act {
 struct Rows {
   int64_t rows, samples, sample_rows, block_rows;
   const int32_t *ends;  // null: samples of sample_rows rows
+  float one;            // 1 (see addRounded)
 };
 
 // First row of sample s (s <= samples); within [0, rows] whatever the entries hold.
@@ -91,10 +92,11 @@ template <int VEC, bool UNIFORM>
 struct Norm {
   static constexpr int kPairs = (VEC + 1) / 2, kGroups = UNIFORM ? 1 : kPairs;
   Two minus_mean[kGroups], rstd[kGroups], gamma[kPairs], beta[kPairs];
+  float one;
   // The activation's argument, rounded after every operation: a value next to the border of relu falls on the same
   // side in the forward pass, in both backward passes and in the formula evaluated step by step.
   __device__ __forceinline__ Two xhat(int j, Two x) const { return (x + minus_mean[UNIFORM ? 0 : j]) * rstd[UNIFORM ? 0 : j]; }
-  __device__ __forceinline__ Two affine(int j, Two xh) const { return xh * gamma[j] + beta[j]; }
+  __device__ __forceinline__ Two affine(int j, Two xh) const { return addRounded(xh * gamma[j], beta[j], one); }
 };
 // value(c) for the channels of pair j of a thread whose first channel is `first`.
 template <int VEC, typename F>
@@ -103,7 +105,8 @@ __device__ __forceinline__ Two ofPair(int first, int j, F value) {
 }
 template <typename T, int VEC, bool UNIFORM>
 __device__ __forceinline__ void loadNorm(Norm<VEC, UNIFORM> &c, const float *mean, const float *rstd, const void *weight,
-                                         const void *bias, bool float_affine, int first, int group_channels) {
+                                         const void *bias, bool float_affine, int first, int group_channels, float one) {
+  c.one = one;
 #pragma unroll
   for (int j = 0; j < Norm<VEC, UNIFORM>::kGroups; ++j) {
     c.minus_mean[j] = ofPair<UNIFORM ? 2 : VEC>(first, j, [&](int ch) { return -mean[(UNIFORM ? first : ch) / group_channels]; });

@@ -266,7 +266,7 @@ normaliseKernel(const T *x, const void *weight, const void *bias, bool float_aff
   forSamples(r, begin, end, [&](int64_t at, int64_t stop, int64_t sample) {
     if (!active) return;
     Norm<VEC, UNIFORM> c;
-    loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, channels / groups);
+    loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, channels / groups, r.one);
     auto put = [&](T *to, const Values<T, VEC> &v) {
       Two o[kPairs];
 #pragma unroll
@@ -313,7 +313,7 @@ gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bo
     for (int j = 0; j < kPairs; ++j) a[j] = b[j] = two(0.0f, 0.0f);
     if (active) {
       Norm<VEC, UNIFORM> c;
-      loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, channels / groups);
+      loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, channels / groups, r.one);
       auto add = [&](const Values<T, VEC> &v, const Values<T, VEC> &g) {
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
@@ -428,7 +428,7 @@ inputGradKernel(const T *dy, const T *x, const void *weight, const void *bias, b
   forSamples(r, begin, end, [&](int64_t at, int64_t stop, int64_t sample) {
     if (!active) return;
     Norm<VEC, UNIFORM> c;
-    loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, group_channels);
+    loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, group_channels, r.one);
     constexpr int kGroups = Norm<VEC, UNIFORM>::kGroups;
     Two minus_m1[kGroups], minus_m2[kGroups];
     const float2 *means = group_means + sample * groups;
@@ -505,7 +505,7 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
     for (int j = 0; j < kPairs; ++j) a[j] = b[j] = minus_k[j] = two(0.0f, 0.0f);
     if (active && rows > 0) {
       if (BACKWARD) {
-        loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, group_channels);
+        loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, group_channels, r.one);
       } else {
         Values<T, VEC> k;
         k.load(x + begin * channels + first);
@@ -589,6 +589,7 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
         }
       }
       if (!BACKWARD) {
+        c.one = r.one;
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
           c.gamma[j] = ofPair<VEC>(first, j, [&](int ch) { return weight ? loadAffine<T>(weight, float_affine, ch) : 1.0f; });
@@ -631,7 +632,7 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
 size_t roundUp(size_t v) { return (v + 255) / 256 * 256; }
 
 Rows rowsOf(const NormProblem &p, const NormPlan &plan) {
-  return Rows{p.rows, p.samples, p.sample_rows, plan.block_rows, p.sample_ends};
+  return Rows{p.rows, p.samples, p.sample_rows, plan.block_rows, p.sample_ends, 1.0f};
 }
 
 char *scratchBase(void *workspace) {
@@ -672,7 +673,7 @@ cudaError_t launchSlices(const NormProblem &p, int columns, const void *output_g
   auto kernel = p.activation == MLUOP_GROUP_NORM_ACT_RELU   ? sliceKernel<T, VEC, MLUOP_GROUP_NORM_ACT_RELU, UNIFORM, BACKWARD>
                 : p.activation == MLUOP_GROUP_NORM_ACT_SILU ? sliceKernel<T, VEC, MLUOP_GROUP_NORM_ACT_SILU, UNIFORM, BACKWARD>
                                                             : sliceKernel<T, VEC, MLUOP_GROUP_NORM_ACT_NONE, UNIFORM, BACKWARD>;
-  const Rows r{p.rows, p.samples, p.sample_rows, 0, p.sample_ends};
+  const Rows r{p.rows, p.samples, p.sample_rows, 0, p.sample_ends, 1.0f};
   kernel<<<grid, kSmallThreads, smem, stream>>>(static_cast<const T *>(output_grad), static_cast<const T *>(input), weight,
                                                 bias, p.float_affine, mean, rstd, r, p.channels, p.groups, l, p.epsilon,
                                                 static_cast<T *>(out), weight_grad, bias_grad, p.float_affine_grad);

@@ -18,7 +18,7 @@
 // 8-bit states: with 10 bytes an element the arithmetic is what has to be short.  It
 // runs on pairs of floats, and the change of the parameter, which no code depends on,
 // takes the approximate reciprocal (2^-22 of it).  Single operations and a correctly
-// rounded quotient took 296 us for 10^8 bfloat16 elements, this form 206 us (1.0 GB).
+// rounded quotient took 296 us for 10^8 bfloat16 elements, this form 210 us (1.0 GB).
 // One block of 256 a warp and five blocks of threads an SM; two or four blocks a warp,
 // their loads ahead of their use, were slower by 4 and 35 %.
 //
@@ -53,7 +53,7 @@ constexpr int kSmallChunk = 1024;  // the same where chunks of 4096 would not fi
 constexpr int kChunk8Bit = 2048;   // 8-bit states: a block of 256 for each warp
 constexpr int kMaxTensors = 480;   // tensors of one launch
 constexpr float kCodeMax = 448.0f;  // largest e4m3 value
-constexpr float kSmallest = 1e-30f;  // below it a block is stored as zeros: 448 / x would leave the float range
+constexpr float kSmallest = 1e-30f;  // below it a block is stored as zeros: 1 / x * 448 would leave the float range
 constexpr float kCodeTiny = 0.001953125f;  // 2^-9, the smallest e4m3 value above zero
 
 struct Constants {
@@ -61,6 +61,7 @@ struct Constants {
   float decay;       // 1 - lr * weight_decay
   float root_scale;  // 1 / sqrt(1 - beta2^t)
   float step_size;   // lr / (1 - beta1^t)
+  float one;         // 1 (see addRounded)
 };
 
 struct TensorTable {
@@ -202,9 +203,11 @@ __device__ __forceinline__ float largest(float a, float b) {
 }
 
 struct Pairs {
+  float one;
   Two beta1, one_minus_beta1, beta2, one_minus_beta2, epsilon, decay, root_scale, minus_step;
   __device__ __forceinline__ explicit Pairs(const Constants &c)
-      : beta1(two(c.beta1, c.beta1)),
+      : one(c.one),
+        beta1(two(c.beta1, c.beta1)),
         one_minus_beta1(two(c.one_minus_beta1, c.one_minus_beta1)),
         beta2(two(c.beta2, c.beta2)),
         one_minus_beta2(two(c.one_minus_beta2, c.one_minus_beta2)),
@@ -215,8 +218,8 @@ struct Pairs {
 };
 // Two elements: m and root (sqrt(v)) are updated in place.  Returns the new parameters.
 __device__ __forceinline__ Two updatePair(Two p, Two g, Two &m, Two &root, const Pairs &c) {
-  m = m * c.beta1 + g * c.one_minus_beta1;
-  const float2 r = split((root * root) * c.beta2 + (g * g) * c.one_minus_beta2);
+  m = addRounded(m * c.beta1, g * c.one_minus_beta1, c.one);
+  const float2 r = split(addRounded((root * root) * c.beta2, (g * g) * c.one_minus_beta2, c.one));
   root = two(__fsqrt_rn(r.x), __fsqrt_rn(r.y));
   float2 d = split(fma(root, c.root_scale, c.epsilon));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.x));
@@ -233,7 +236,7 @@ __device__ __forceinline__ BlockScale blockScale(float lane_largest) {
   const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lane_largest)));
   BlockScale s{0.0f, 0.0f};
   if (!(most < kSmallest)) {
-    s.inverse = __fdiv_rn(kCodeMax, most);
+    s.inverse = __fmul_rn(__frcp_rn(most), kCodeMax);
     s.scale = __fmul_rn(most, 1.0f / kCodeMax);
   }
   return s;
@@ -393,6 +396,7 @@ cudaError_t launchMultiTensorAdamW(const AdamWProblem &p, cudaStream_t stream) {
   t.c.beta2 = (float)p.beta2;
   t.c.one_minus_beta2 = (float)(1.0 - p.beta2);
   t.c.epsilon = (float)p.epsilon;
+  t.c.one = 1.0f;
   t.c.decay = (float)(1.0 - p.lr * p.weight_decay);
   t.c.step_size = (float)(p.lr / (1.0 - std::pow(p.beta1, (double)p.step)));
   t.c.root_scale = (float)(1.0 / std::sqrt(1.0 - std::pow(p.beta2, (double)p.step)));
