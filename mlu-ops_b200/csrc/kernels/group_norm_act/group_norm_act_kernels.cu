@@ -32,6 +32,7 @@
 #include <algorithm>
 #include <numeric>
 
+#include "core/launch.cuh"
 #include "core/trace.h"
 #include "core/type.h"
 #include "kernels/group_norm_act/group_norm_act_device.cuh"
@@ -130,6 +131,7 @@ __device__ __forceinline__ void forSamples(const Rows &r, int64_t begin, int64_t
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, 4)
 statisticsKernel(const T *x, Rows r, int channels, Lanes l, float2 *partial) {
+  letNextKernelStart();
   extern __shared__ __align__(16) float2 scratch[];
   constexpr int kPairs = (VEC + 1) / 2;
   const int column = threadIdx.x % l.columns, row = threadIdx.x / l.columns;
@@ -215,6 +217,7 @@ struct SampleSlots {
 // Pass 2 forward: one block per (sample, group).  The blocks' means are joined as distances from the first one.
 __global__ void __launch_bounds__(kThreads)
 joinStatisticsKernel(const float2 *partial, Rows r, int channels, int groups, float epsilon, float *mean, float *rstd) {
+  letNextKernelStart();
   __shared__ double2 scratch[kThreads / 32];
   const int64_t sample = blockIdx.x / groups;
   const int group = blockIdx.x % groups, group_channels = channels / groups;
@@ -222,6 +225,7 @@ joinStatisticsKernel(const float2 *partial, Rows r, int channels, int groups, fl
   const int width = group_channels < kThreads ? group_channels : kThreads, depth = kThreads / width;
   const int c0 = threadIdx.x % width, d = threadIdx.x / width;
   double a = 0.0, b = 0.0, ref = 0.0;
+  waitForKernelBefore();
   if (s.last >= s.first && d < depth) {
     const float2 *from = partial + sample * channels + (int64_t)group * group_channels;
     ref = from[(int64_t)s.first * channels].x;
@@ -263,6 +267,7 @@ normaliseKernel(const T *x, const void *weight, const void *bias, bool float_aff
   const int64_t begin = (int64_t)(gridDim.x - 1 - blockIdx.x) * r.block_rows;
   const int64_t end = begin + r.block_rows < r.rows ? begin + r.block_rows : r.rows;
   const int64_t step = (int64_t)l.row_threads * channels;
+  waitForKernelBefore();
   forSamples(r, begin, end, [&](int64_t at, int64_t stop, int64_t sample) {
     if (!active) return;
     Norm<VEC, UNIFORM> c;
@@ -299,6 +304,7 @@ template <typename T, int VEC, int ACT, bool UNIFORM>
 __global__ void __launch_bounds__(kThreads, 3)
 gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bool float_affine, const float *mean,
                const float *rstd, Rows r, int channels, int groups, Lanes l, float2 *partial) {
+  letNextKernelStart();
   extern __shared__ __align__(16) float2 scratch[];
   constexpr int kPairs = (VEC + 1) / 2;
   const int column = threadIdx.x % l.columns, row = threadIdx.x / l.columns;
@@ -356,6 +362,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 joinGradSumsKernel(const float2 *partial, const void *weight, bool float_affine, Rows r, int channels, int groups,
                    float2 *sample_sums, float2 *group_means) {
+  letNextKernelStart();
   __shared__ double2 scratch[kThreads / 32], lanes[kThreads];
   const int64_t sample = blockIdx.x / groups;
   const int group = blockIdx.x % groups, group_channels = channels / groups;
@@ -364,6 +371,7 @@ joinGradSumsKernel(const float2 *partial, const void *weight, bool float_affine,
   const int width = group_channels < 32 ? group_channels : 32, depth = kThreads / width;
   const int c = threadIdx.x % width, d = threadIdx.x / width;
   double m1 = 0.0, m2 = 0.0;
+  waitForKernelBefore();
   for (int base = 0; base < group_channels; base += width) {
     const int channel = group * group_channels + base + c;
     const bool active = d < depth && base + c < group_channels;
@@ -407,6 +415,7 @@ inputGradKernel(const T *dy, const T *x, const void *weight, const void *bias, b
   const int column = threadIdx.x % l.columns, row = threadIdx.x / l.columns;
   const int first = (blockIdx.y * l.columns + column) * VEC, group_channels = channels / groups;
   const bool active = row < l.row_threads && first < channels;
+  waitForKernelBefore();
   if (weight_grad) {
     const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     const int64_t all = (int64_t)gridDim.x * gridDim.y * kThreads;
@@ -699,17 +708,16 @@ cudaError_t forward(const NormProblem &p, const NormPlan &plan, const void *inpu
   if (err != cudaSuccess) return err;
   if (p.samples > 0) {
     trace::Scope scope("groupNormJoinKernel", stream);
-    joinStatisticsKernel<<<(unsigned)(p.samples * p.groups), kThreads, 0, stream>>>(partial, r, p.channels, p.groups,
-                                                                                    p.epsilon, mean, rstd);
+    err = launchAfterKernel(joinStatisticsKernel, dim3((unsigned)(p.samples * p.groups)), dim3(kThreads), 0, stream, partial,
+                            r, p.channels, p.groups, p.epsilon, mean, rstd);
   }
-  err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   trace::Scope scope("groupNormNormaliseKernel", stream, 2 * rowBytes(p));
   auto kernel = p.activation == MLUOP_GROUP_NORM_ACT_RELU   ? normaliseKernel<T, VEC, MLUOP_GROUP_NORM_ACT_RELU, UNIFORM>
                 : p.activation == MLUOP_GROUP_NORM_ACT_SILU ? normaliseKernel<T, VEC, MLUOP_GROUP_NORM_ACT_SILU, UNIFORM>
                                                             : normaliseKernel<T, VEC, MLUOP_GROUP_NORM_ACT_NONE, UNIFORM>;
-  kernel<<<grid, kThreads, 0, stream>>>(x, weight, bias, p.float_affine, mean, rstd, r, p.channels, p.groups, l, y);
-  return cudaGetLastError();
+  return launchAfterKernel(kernel, grid, dim3(kThreads), 0, stream, x, weight, bias, p.float_affine, mean, rstd, r,
+                           p.channels, p.groups, l, y);
 }
 
 template <typename T, int VEC, bool UNIFORM, int ACT>
@@ -734,16 +742,14 @@ cudaError_t backward(const NormProblem &p, const NormPlan &plan, const void *out
   if (err != cudaSuccess) return err;
   if (p.samples > 0) {
     trace::Scope scope("groupNormGradJoinKernel", stream);
-    joinGradSumsKernel<T><<<(unsigned)(p.samples * p.groups), kThreads, 0, stream>>>(
-        partial, weight, p.float_affine, r, p.channels, p.groups, sample_sums, group_means);
+    err = launchAfterKernel(joinGradSumsKernel<T>, dim3((unsigned)(p.samples * p.groups)), dim3(kThreads), 0, stream, partial,
+                            weight, p.float_affine, r, p.channels, p.groups, sample_sums, group_means);
   }
-  err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   trace::Scope scope("groupNormInputGradKernel", stream, 3 * rowBytes(p));
-  inputGradKernel<T, VEC, ACT, UNIFORM><<<grid, kThreads, 0, stream>>>(
-      dy, x, weight, bias, p.float_affine, mean, rstd, sample_sums, group_means, r, p.channels, p.groups, l,
-      static_cast<T *>(input_grad), weight_grad, bias_grad, p.float_affine_grad);
-  return cudaGetLastError();
+  return launchAfterKernel(inputGradKernel<T, VEC, ACT, UNIFORM>, grid, dim3(kThreads), 0, stream, dy, x, weight, bias,
+                           p.float_affine, mean, rstd, sample_sums, group_means, r, p.channels, p.groups, l,
+                           static_cast<T *>(input_grad), weight_grad, bias_grad, p.float_affine_grad);
 }
 
 template <typename T, int VEC, bool UNIFORM, typename... Args>

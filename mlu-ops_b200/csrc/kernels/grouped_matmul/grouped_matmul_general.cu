@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "core/convert.cuh"
+#include "core/launch.cuh"
 #include "core/pair.cuh"
 #include "core/trace.h"
 #include "core/type.h"
@@ -98,6 +99,7 @@ template <typename T, typename OutT, int MODE, int VEC>
 __global__ void __launch_bounds__(kThreads)
 generalKernel(const T *a, const T *b, const int32_t *ends, OutT *c, float *partial, int64_t rows, int groups, int ci,
               int co, int64_t chunk_rows, bool vector_out) {
+  if (MODE == kBackwardWeight) letNextKernelStart();
   __shared__ GroupMap map;
   // read as 16-byte vectors: rows are multiples of 16 bytes
   __shared__ alignas(16) float as[kK][kM + kPad], bs[kK][kN + kPad];
@@ -213,6 +215,7 @@ addChunksKernel(const float *partial, const int32_t *ends, OutT *c, int64_t rows
                 int64_t chunk_rows) {
   __shared__ GroupMap map;
   buildGroupMap<true>(map, ends, groups, rows, chunk_rows, 1);
+  waitForKernelBefore();
   for (int g = 0; g < groups; ++g) {
     const int first = map.slot[g], chunks = map.slot[g + 1] - first;
     if (chunks < 2) continue;
@@ -308,12 +311,12 @@ cudaError_t launchAddChunks(const Problem &p, const WeightGradPlan &plan, const 
     const int64_t threads = vectors ? elements / 4 : elements;
     const unsigned grid = (unsigned)std::min<int64_t>(8 * p.sm_count, (threads + kThreads - 1) / kThreads);
     auto kernel = vectors ? addChunksKernel<OutT, 4> : addChunksKernel<OutT, 1>;
-    kernel<<<grid, kThreads, 0, stream>>>(partial, ends, out, p.rows, p.groups, elements, plan.chunk_rows);
+    return launchAfterKernel(kernel, dim3(grid), dim3(kThreads), 0, stream, partial, ends, out, p.rows, p.groups, elements,
+                             plan.chunk_rows);
   };
-  if (p.float_weight_grad || p.dtype == MLUOP_DTYPE_FLOAT) launch(static_cast<float *>(c));
-  else if (p.dtype == MLUOP_DTYPE_HALF) launch(static_cast<__half *>(c));
-  else launch(static_cast<__nv_bfloat16 *>(c));
-  return cudaGetLastError();
+  if (p.float_weight_grad || p.dtype == MLUOP_DTYPE_FLOAT) return launch(static_cast<float *>(c));
+  if (p.dtype == MLUOP_DTYPE_HALF) return launch(static_cast<__half *>(c));
+  return launch(static_cast<__nv_bfloat16 *>(c));
 }
 
 cudaError_t launchGeneral(const Problem &p, const void *a, const void *b, const int32_t *ends, void *c, void *workspace,

@@ -38,6 +38,7 @@
 #include <cstdlib>
 
 #include "core/convert.cuh"
+#include "core/launch.cuh"
 #include "core/trace.h"
 #include "kernels/grouped_matmul/grouped_matmul_device.cuh"
 #include "kernels/grouped_matmul/grouped_matmul_kernels.h"
@@ -309,6 +310,7 @@ __device__ __forceinline__ void writeSums(bool have, unsigned tmem, unsigned cha
 template <int MODE, int CTAS, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
 groupedTcgen05Kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+  if (MODE == kBackwardWeight) letNextKernelStart();
   using Cfg = Config<CTAS, BN>;
   constexpr int S = Cfg::kStages;
   constexpr bool kWeight = MODE == kBackwardWeight;
@@ -347,6 +349,7 @@ groupedTcgen05Kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   if (CTAS == 2) clusterSync();  // both blocks' tensor memory is there before the first MMA writes to it
   tcFenceAfter();
   const unsigned tmem_base = tmem_base_s;
+  if (kWeight) waitForKernelBefore();  // the one that writes the groups' tensor maps
   const int units = map.first[p.groups + 1];
   const int first_unit = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
   volatile int *abort_flag = &abort_s;
@@ -527,6 +530,7 @@ groupedTcgen05Kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 __global__ void __launch_bounds__(kThreads)
 groupMapsKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const int32_t *ends,
                 int groups, int64_t rows, CUtensorMap *out) {
+  letNextKernelStart();
   __shared__ GroupMap map;
   buildGroupMap<true>(map, ends, groups, rows, rows, 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -581,14 +585,16 @@ cudaError_t launch(const Problem &p, const CUtensorMap &a, const CUtensorMap &b,
   auto kernel = groupedTcgen05Kernel<MODE, CTAS, BN>;
   static std::atomic<int> known_clusters{0};  // clusters of this kernel that run at a time (all devices are alike)
   cudaLaunchConfig_t config{};
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = CTAS;
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = CTAS;
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = Cfg::kSmemBytes;
   config.stream = stream;
-  config.attrs = &attribute;
+  config.attrs = attributes;
   config.numAttrs = 1;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::kSmemBytes);
   if (err != cudaSuccess) return err;
@@ -610,6 +616,7 @@ cudaError_t launch(const Problem &p, const CUtensorMap &a, const CUtensorMap &b,
                      : MODE == kBackwardInput ? "groupedTcgen05Kernel:input_grad"
                                               : "groupedTcgen05Kernel:weight_grad",
                      stream, 2.0 * (rows * (p.ci + p.co) + (double)p.groups * p.ci * p.co), 2.0 * rows * p.ci * p.co);
+  if (MODE == kBackwardWeight) config.numAttrs = 2;  // it follows the kernel that writes the groups' tensor maps
   return cudaLaunchKernelEx(&config, kernel, a, b, params);
 }
 
