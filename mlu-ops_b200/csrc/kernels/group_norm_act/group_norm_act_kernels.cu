@@ -301,7 +301,7 @@ normaliseKernel(const T *x, const void *weight, const void *bias, bool float_aff
 
 // Pass 1 backward: partial[slot][channel] = (sum du, sum du xhat) of the block's rows of a sample.
 template <typename T, int VEC, int ACT, bool UNIFORM>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 2)
 gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bool float_affine, const float *mean,
                const float *rstd, Rows r, int channels, int groups, Lanes l, float2 *partial) {
   letNextKernelStart();
@@ -332,7 +332,7 @@ gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bo
       int left = (int)(stop - at) - row;
       const int64_t offset = (at + row) * channels + first;
       const T *from = x + offset, *from_g = dy + offset;
-      constexpr int kRows = kUnroll / 2;
+      constexpr int kRows = kUnroll;
       for (; left > (kRows - 1) * l.row_threads; left -= kRows * l.row_threads, from += kRows * step, from_g += kRows * step) {
         Values<T, VEC> v[kRows], g[kRows];
 #pragma unroll
@@ -343,7 +343,7 @@ gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bo
 #pragma unroll
         for (int u = 0; u < kRows; ++u) add(v[u], g[u]);
       }
-      if (left > 0) {
+      for (; left > 0; left -= l.row_threads, from += step, from_g += step) {
         Values<T, VEC> v, g;
         v.load(from);
         g.load(from_g);
@@ -407,7 +407,7 @@ joinGradSumsKernel(const float2 *partial, const void *weight, bool float_affine,
 
 // Pass 3 backward: the input gradient; the first blocks also add the samples' sums to the affine gradients.
 template <typename T, int VEC, int ACT, bool UNIFORM>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 2)
 inputGradKernel(const T *dy, const T *x, const void *weight, const void *bias, bool float_affine, const float *mean,
                 const float *rstd, const float2 *sample_sums, const float2 *group_means, Rows r, int channels,
                 int groups, Lanes l, T *dx, void *weight_grad, void *bias_grad, bool float_affine_grad) {
@@ -461,7 +461,7 @@ inputGradKernel(const T *dy, const T *x, const void *weight, const void *bias, b
     const int64_t offset = (at + row) * channels + first;
     const T *from = x + offset, *from_g = dy + offset;
     T *to = dx + offset;
-    constexpr int kRows = kUnroll / 2;
+    constexpr int kRows = kUnroll;
     for (; left > (kRows - 1) * l.row_threads; left -= kRows * l.row_threads, from += kRows * step, from_g += kRows * step, to += kRows * step) {
       Values<T, VEC> v[kRows], g[kRows];
 #pragma unroll
@@ -472,7 +472,7 @@ inputGradKernel(const T *dy, const T *x, const void *weight, const void *bias, b
 #pragma unroll
       for (int u = 0; u < kRows; ++u) put(to + u * step, v[u], g[u]);
     }
-    if (left > 0) {
+    for (; left > 0; left -= l.row_threads, from += step, from_g += step, to += step) {
       Values<T, VEC> v, g;
       v.load(from);
       g.load(from_g);
@@ -786,9 +786,9 @@ NormPlan planNorm(const NormProblem &p, bool backward, bool vectors) {
   plan.column_threads = std::min(columns, kThreads);
   plan.column_tiles = (columns + plan.column_threads - 1) / plan.column_threads;
   plan.row_threads = kThreads / plan.column_threads;
-  // as many blocks as run at a time (four to an SM forward, three backward), so that each has long runs of rows, and at
+  // as many blocks as run at a time (four to an SM forward, two backward), so that each has long runs of rows, and at
   // least one unrolled turn for each block
-  const int64_t wanted = std::max<int64_t>(1, (int64_t)(backward ? 3 : 4) * p.sm_count / plan.column_tiles);
+  const int64_t wanted = std::max<int64_t>(1, (int64_t)(backward ? 2 : 4) * p.sm_count / plan.column_tiles);
   const int64_t turn = (int64_t)kUnroll * plan.row_threads;
   plan.block_rows = std::max<int64_t>(1, (p.rows + wanted - 1) / wanted);
   plan.block_rows = (plan.block_rows + turn - 1) / turn * turn;
