@@ -772,28 +772,27 @@ def _address(handle, name, t):
 
 
 class _CallPlan:
-    """Descriptors (d: their addresses, in the order of `specs`; None stays None) and workspace bytes of a call."""
+    """Descriptors of the tensors of a call (d: their addresses; None stays None) and its workspace bytes."""
     __slots__ = ("descs", "d", "workspace")
 
-    def __init__(self, specs):
+    def __init__(self, handle, key, specs, query=None):
         self.descs = [None if s is None else TensorDesc(LAYOUT_ARRAY, _dtype_code(s[0]), tuple(s[1])) for s in specs]
         self.d = [None if t is None else t.ptr.value for t in self.descs]
         self.workspace = 0
-
-
-def _call_plan(handle, key, specs, query=None):
-    """The handle's plan for `key`; a new one describes `specs()` and asks `query(plan, size)` for its workspace."""
-    plan = handle.plans.get(key)
-    if plan is None:
-        plan = _CallPlan(specs())
         if query is not None:
             size = _szt(0)
-            query(plan, size)
-            plan.workspace = size.value
+            query(self.d, ctypes.byref(size))
+            self.workspace = size.value
         if len(handle.plans) >= 512:  # shapes that change from step to step do not pile up
             handle.plans.clear()
-        handle.plans[key] = plan
-    return plan
+        handle.plans[key] = self
+
+
+def _on_own_queue(handle):
+    """Whether tensors of the current stream's memory pool are the handle's queue's to use at once."""
+    import torch
+    return _guards is None and (handle.device < 0
+                                or torch._C._cuda_getCurrentRawStream(handle.device) == (handle.stream or 0))
 
 
 def _new(handle, like, shape, dtype):
@@ -801,23 +800,14 @@ def _new(handle, like, shape, dtype):
     pool, and kept until the current stream is done with it too."""
     if _guards is not None:
         return _guards.empty(shape, dtype, like.device)
-    import torch
-    if handle.device < 0 or torch._C._cuda_getCurrentRawStream(handle.device) == (handle.stream or 0):
+    if _on_own_queue(handle):
         return like.new_empty(shape, dtype=dtype)
+    import torch
     current = torch.cuda.current_stream(handle.device)
     with torch.cuda.stream(torch.cuda.ExternalStream(handle.stream or 0, device=handle.device)):
         t = like.new_empty(shape, dtype=dtype)
     t.record_stream(current)
     return t
-
-
-def _workspace(handle, like, nbytes):
-    """(tensor, address) of a workspace; (None, None) if none is needed."""
-    import torch
-    if nbytes == 0:
-        return None, None
-    t = _new(handle, like, (nbytes,), torch.uint8)
-    return t, t.data_ptr()
 
 
 def _spec(t):
@@ -847,24 +837,32 @@ def group_norm_act_forward(handle, input, weight, bias, num_groups, epsilon=1e-5
     p_w = None if weight is None else _address(handle, "weight", weight)
     p_b = None if bias is None else _address(handle, "bias", bias)
     p_e = None if sample_ends is None else _address(handle, "sample_ends", sample_ends)
-    num_groups = int(num_groups)
-    stats = ((input.shape[0] if sample_ends is None else sample_ends.shape[0]), num_groups)
-    if out is None:
-        out = _new(handle, input, input.shape, input.dtype)
-    mean, rstd = _new(handle, input, stats, torch.float32), _new(handle, input, stats, torch.float32)
-    p_y = _address(handle, "out", out)
-    specs = lambda: [_spec(t) for t in (input, weight, bias, sample_ends, out)] + [(torch.float32, stats)]  # noqa: E731
-    plan = _call_plan(handle, ("norm", num_groups, input.shape, input.dtype, out.shape, out.dtype, _spec(weight),
-                               _spec(bias), _spec(sample_ends)), specs,
-                      lambda plan, size: check("mluOpGetGroupNormActForwardWorkspaceSize",
+    stats = ((input if sample_ends is None else sample_ends).shape[0], int(num_groups))
+    if _on_own_queue(handle):
+        y = torch.empty_like(input) if out is None else out
+        mean = input.new_empty(stats, dtype=torch.float32)
+        rstd = torch.empty_like(mean)
+    else:
+        y = _new(handle, input, input.shape, input.dtype) if out is None else out
+        mean, rstd = _new(handle, input, stats, torch.float32), _new(handle, input, stats, torch.float32)
+    p_y = y.data_ptr() if out is None else _address(handle, "out", out)
+    key = ("norm", num_groups, input.shape, input.dtype, None if weight is None else (weight.shape, weight.dtype),
+           None if bias is None else (bias.shape, bias.dtype), None if sample_ends is None else (sample_ends.shape, sample_ends.dtype),
+           None if out is None else (out.shape, out.dtype))
+    plan = handle.plans.get(key)
+    if plan is None:
+        plan = _CallPlan(handle, key, [_spec(t) for t in (input, weight, bias, sample_ends, y)] + [(torch.float32, stats)],
+                         lambda d, size: check("mluOpGetGroupNormActForwardWorkspaceSize",
                                                lib().mluOpGetGroupNormActForwardWorkspaceSize(
-                                                   handle.ptr, plan.d[0], plan.d[3], num_groups, ctypes.byref(size))))
+                                                   handle.ptr, d[0], d[3], stats[1], size)))
     d_x, d_w, d_b, d_e, d_y, d_m = plan.d
-    workspace, p_s = _workspace(handle, input, plan.workspace)
-    check("mluOpGroupNormActForward",
-          lib().mluOpGroupNormActForward(handle.ptr, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, num_groups, epsilon, act,
-                                         p_s, plan.workspace, d_y, p_y, d_m, mean.data_ptr(), d_m, rstd.data_ptr()))
-    return out, mean, rstd
+    workspace = _new(handle, input, (plan.workspace,), torch.uint8) if plan.workspace else None
+    st = lib().mluOpGroupNormActForward(handle.ptr, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, stats[1], epsilon, act,
+                                        workspace.data_ptr() if plan.workspace else None, plan.workspace, d_y, p_y, d_m,
+                                        mean.data_ptr(), d_m, rstd.data_ptr())
+    if st:
+        check("mluOpGroupNormActForward", st)
+    return y, mean, rstd
 
 
 def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd, num_groups, activation="none",
@@ -885,25 +883,31 @@ def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd
     p_m, p_r = _address(handle, "mean", mean), _address(handle, "rstd", rstd)
     num_groups = int(num_groups)
     if out is None:
-        out = _new(handle, input, input.shape, input.dtype)
+        out = torch.empty_like(input) if _on_own_queue(handle) else _new(handle, input, input.shape, input.dtype)
     p_o = _address(handle, "out", out)
     weight_grad = bias_grad = p_wg = p_bg = None
     if affine_grad:
         weight_grad = _new(handle, input, input.shape[-1:], affine_grad_dtype or torch.float32)
-        bias_grad = _new(handle, input, input.shape[-1:], affine_grad_dtype or torch.float32)
+        bias_grad = torch.empty_like(weight_grad) if _on_own_queue(handle) else _new(handle, input, input.shape[-1:], weight_grad.dtype)
         p_wg, p_bg = weight_grad.data_ptr(), bias_grad.data_ptr()
-    tensors = (output_grad, input, weight, bias, sample_ends, mean, rstd, out, weight_grad, bias_grad)
-    plan = _call_plan(handle, ("norm_grad", num_groups) + tuple([_spec(t) for t in tensors]),
-                      lambda: [_spec(t) for t in tensors],
-                      lambda plan, size: check("mluOpGetGroupNormActBackwardWorkspaceSize",
+    key = ("norm_grad", num_groups, input.shape, input.dtype, output_grad.shape, output_grad.dtype, out.shape, out.dtype,
+           mean.shape, mean.dtype, rstd.shape, rstd.dtype, None if weight is None else (weight.shape, weight.dtype),
+           None if bias is None else (bias.shape, bias.dtype), None if sample_ends is None else (sample_ends.shape, sample_ends.dtype),
+           weight_grad.dtype if affine_grad else None)
+    plan = handle.plans.get(key)
+    if plan is None:
+        plan = _CallPlan(handle, key, [_spec(t) for t in (output_grad, input, weight, bias, sample_ends, mean, rstd, out,
+                                                          weight_grad, bias_grad)],
+                         lambda d, size: check("mluOpGetGroupNormActBackwardWorkspaceSize",
                                                lib().mluOpGetGroupNormActBackwardWorkspaceSize(
-                                                   handle.ptr, plan.d[1], plan.d[4], num_groups, ctypes.byref(size))))
+                                                   handle.ptr, d[1], d[4], num_groups, size)))
     d_g, d_x, d_w, d_b, d_e, d_m, d_r, d_o, d_wg, d_bg = plan.d
-    workspace, p_s = _workspace(handle, input, plan.workspace)
-    check("mluOpGroupNormActBackward",
-          lib().mluOpGroupNormActBackward(handle.ptr, d_g, p_g, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, d_m, p_m, d_r,
-                                          p_r, num_groups, act, p_s, plan.workspace, d_o, p_o, d_wg, p_wg, d_bg,
-                                          p_bg))
+    workspace = _new(handle, input, (plan.workspace,), torch.uint8) if plan.workspace else None
+    st = lib().mluOpGroupNormActBackward(handle.ptr, d_g, p_g, d_x, p_x, d_w, p_w, d_b, p_b, d_e, p_e, d_m, p_m, d_r, p_r,
+                                         num_groups, act, workspace.data_ptr() if plan.workspace else None, plan.workspace,
+                                         d_o, p_o, d_wg, p_wg, d_bg, p_bg)
+    if st:
+        check("mluOpGroupNormActBackward", st)
     return out, weight_grad, bias_grad
 
 
@@ -997,6 +1001,25 @@ class MultiTensorAdamW:
                                           epsilon, weight_decay, int(step), _ptr(grad_scale), _ptr(schedule)))
 
 
+def _grouped_rows_call(name, handle, rows, weight, group_ends, columns, out):
+    """The forward product and the input gradient: rows [R,K] times each group's matrix into [R, columns]."""
+    p_x, p_w, p_e = (_address(handle, "the row matrix", rows), _address(handle, "weight", weight),
+                     _address(handle, "group_ends", group_ends))
+    if out is None:
+        out = _new(handle, rows, (rows.shape[0], columns), rows.dtype)
+    p_y = _address(handle, "out", out)
+    key = ("product", rows.shape, rows.dtype, weight.shape, weight.dtype, group_ends.shape, group_ends.dtype, out.shape,
+           out.dtype)
+    plan = handle.plans.get(key)
+    if plan is None:
+        plan = _CallPlan(handle, key, [_spec(t) for t in (rows, weight, group_ends, out)])
+    d_x, d_w, d_e, d_y = plan.d
+    st = getattr(lib(), name)(handle.ptr, d_x, p_x, d_w, p_w, d_e, p_e, d_y, p_y)
+    if st:
+        check(name, st)
+    return out
+
+
 def grouped_matmul_forward(handle, input, weight, group_ends, out=None):
     """output [rows,Co] with output[r] = input[r] @ weight[g] for the rows r of group g, through
     mluOpGroupedMatMulForward.
@@ -1005,56 +1028,36 @@ def grouped_matmul_forward(handle, input, weight, group_ends, out=None):
     [G] on the device: group g's rows end there, the next group's begin.  Rows behind the last
     group's end: zeros.
     """
-    p_x, p_w, p_e = (_address(handle, "input", input), _address(handle, "weight", weight),
-                     _address(handle, "group_ends", group_ends))
-    if out is None:
-        out = _new(handle, input, (input.shape[0], weight.shape[-1]), input.dtype)
-    p_y = _address(handle, "out", out)
-    tensors = (input, weight, group_ends, out)
-    plan = _call_plan(handle, ("product", input.shape, input.dtype, weight.shape, weight.dtype, group_ends.shape,
-                               group_ends.dtype, out.shape, out.dtype), lambda: [_spec(t) for t in tensors])
-    d_x, d_w, d_e, d_y = plan.d
-    check("mluOpGroupedMatMulForward",
-          lib().mluOpGroupedMatMulForward(handle.ptr, d_x, p_x, d_w, p_w, d_e, p_e, d_y, p_y))
-    return out
+    return _grouped_rows_call("mluOpGroupedMatMulForward", handle, input, weight, group_ends, weight.shape[-1], out)
 
 
 def grouped_matmul_backward_input(handle, output_grad, weight, group_ends, out=None):
     """input_grad [rows,Ci] with input_grad[r] = output_grad[r] @ weight[g].T through
     mluOpGroupedMatMulBackwardInput (the forward call's arguments)."""
-    p_g, p_w, p_e = (_address(handle, "output_grad", output_grad), _address(handle, "weight", weight),
-                     _address(handle, "group_ends", group_ends))
-    if out is None:
-        out = _new(handle, output_grad, (output_grad.shape[0], weight.shape[-2]), output_grad.dtype)
-    p_x = _address(handle, "out", out)
-    tensors = (output_grad, weight, group_ends, out)
-    plan = _call_plan(handle, ("product", output_grad.shape, output_grad.dtype, weight.shape, weight.dtype,
-                               group_ends.shape, group_ends.dtype, out.shape, out.dtype),
-                      lambda: [_spec(t) for t in tensors])
-    d_g, d_w, d_e, d_x = plan.d
-    check("mluOpGroupedMatMulBackwardInput",
-          lib().mluOpGroupedMatMulBackwardInput(handle.ptr, d_g, p_g, d_w, p_w, d_e, p_e, d_x, p_x))
-    return out
+    return _grouped_rows_call("mluOpGroupedMatMulBackwardInput", handle, output_grad, weight, group_ends, weight.shape[-2], out)
 
 
 def grouped_matmul_backward_weight(handle, input, output_grad, group_ends, dtype=None, out=None):
     """weight_grad [G,Ci,Co] with weight_grad[g] = input[rows of g].T @ output_grad[rows of g] through
     mluOpGroupedMatMulBackwardWeight; dtype: input's (default) or float32."""
+    import torch
     p_x, p_g, p_e = (_address(handle, "input", input), _address(handle, "output_grad", output_grad),
                      _address(handle, "group_ends", group_ends))
     if out is None:
         out = _new(handle, input, (group_ends.shape[0], input.shape[-1], output_grad.shape[-1]), dtype or input.dtype)
     p_w = _address(handle, "out", out)
-    tensors = (input, output_grad, group_ends, out)
-    plan = _call_plan(handle, ("product_weight", input.shape, input.dtype, output_grad.shape, output_grad.dtype,
-                               group_ends.shape, group_ends.dtype, out.shape, out.dtype),
-                      lambda: [_spec(t) for t in tensors],
-                      lambda plan, size: check("mluOpGetGroupedMatMulBackwardWeightWorkspaceSize",
+    key = ("product_weight", input.shape, input.dtype, output_grad.shape, output_grad.dtype, group_ends.shape,
+           group_ends.dtype, out.shape, out.dtype)
+    plan = handle.plans.get(key)
+    if plan is None:
+        plan = _CallPlan(handle, key, [_spec(t) for t in (input, output_grad, group_ends, out)],
+                         lambda d, size: check("mluOpGetGroupedMatMulBackwardWeightWorkspaceSize",
                                                lib().mluOpGetGroupedMatMulBackwardWeightWorkspaceSize(
-                                                   handle.ptr, plan.d[0], plan.d[1], plan.d[3], ctypes.byref(size))))
+                                                   handle.ptr, d[0], d[1], d[3], size)))
     d_x, d_g, d_e, d_w = plan.d
-    workspace, p_s = _workspace(handle, input, plan.workspace)
-    check("mluOpGroupedMatMulBackwardWeight",
-          lib().mluOpGroupedMatMulBackwardWeight(handle.ptr, d_x, p_x, d_g, p_g, d_e, p_e, p_s, plan.workspace, d_w,
-                                                 p_w))
+    workspace = _new(handle, input, (plan.workspace,), torch.uint8)
+    st = lib().mluOpGroupedMatMulBackwardWeight(handle.ptr, d_x, p_x, d_g, p_g, d_e, p_e, workspace.data_ptr(),
+                                                plan.workspace, d_w, p_w)
+    if st:
+        check("mluOpGroupedMatMulBackwardWeight", st)
     return out
