@@ -7,6 +7,7 @@
 
 #include "core/context.h"
 #include "core/logging.h"
+#include "core/overlap.h"
 #include "core/tensor.h"
 #include "kernels/group_norm_act/group_norm_act_kernels.h"
 
@@ -21,6 +22,9 @@ bool isRowType(mluOpDataType_t t) {
 }
 
 bool aligned(const void *p, size_t to) { return reinterpret_cast<size_t>(p) % to == 0; }
+
+// In place, or nowhere on the other tensor.
+bool sameOrApart(const void *a, const void *b, size_t bytes) { return a == b || !mluop::overlap(a, bytes, b, bytes); }
 
 bool sameDims(const mluOpTensorDescriptor_t a, const mluOpTensorDescriptor_t b) {
   if (a->getDim() != b->getDim()) return false;
@@ -55,7 +59,8 @@ mluOpStatus_t makeProblem(const std::string &api, mluOpHandle_t handle, const ml
   }
   p->samples = input_desc->getDimIndex(0);
   p->sample_rows = inner;
-  if (sample_ends_desc != nullptr) {
+  p->ragged = sample_ends_desc != nullptr;
+  if (p->ragged) {
     PARAM_CHECK_EQ(api, dim, 2);
     PARAM_CHECK_EQ(api, sample_ends_desc->getDim(), 1);
     PARAM_CHECK(api, sample_ends_desc->getDtype() == MLUOP_DTYPE_INT32);
@@ -187,7 +192,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActForward(
   RETURN_UNLESS_OK(affineCheck(api, p, weight_desc, bias_desc, &p.float_affine));
   RETURN_UNLESS_OK(rowTensorCheck(api, input_desc, output_desc));
   RETURN_UNLESS_OK(statisticsCheck(api, p, mean_desc, rstd_desc));
-  PARAM_CHECK(api, std::isfinite(epsilon) && epsilon > 0.0);
+  PARAM_CHECK(api, std::isfinite((float)epsilon) && (float)epsilon > 0.0f);
   PARAM_CHECK(api, isActivation(activation));
   if (p.rows == 0 && p.samples == 0) {
     VLOG(5) << api << " Skip zero element tensor.";
@@ -197,6 +202,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActForward(
   if (p.rows > 0) {
     PARAM_CHECK(api, input != nullptr && aligned(input, size));
     PARAM_CHECK(api, output != nullptr && aligned(output, size));
+    PARAM_CHECK(api, sameOrApart(output, input, mluop::denseBytes(input_desc)));
     if (weight_desc != nullptr) {
       PARAM_CHECK(api, weight != nullptr && aligned(weight, affine_size));
       PARAM_CHECK(api, bias != nullptr && aligned(bias, affine_size));
@@ -264,6 +270,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActBackward(
     PARAM_CHECK(api, output_grad != nullptr && aligned(output_grad, size));
     PARAM_CHECK(api, input != nullptr && aligned(input, size));
     PARAM_CHECK(api, input_grad != nullptr && aligned(input_grad, size));
+    PARAM_CHECK(api, sameOrApart(input_grad, output_grad, mluop::denseBytes(input_desc)));
+    PARAM_CHECK(api, sameOrApart(input_grad, input, mluop::denseBytes(input_desc)));
     if (weight_desc != nullptr) {
       PARAM_CHECK(api, weight != nullptr && aligned(weight, affine_size));
       PARAM_CHECK(api, bias != nullptr && aligned(bias, affine_size));

@@ -119,6 +119,109 @@ __device__ __forceinline__ void loadNorm(Norm<VEC, UNIFORM> &c, const float *mea
   }
 }
 
+// A block's threads: `columns` side by side on a row, `row_threads` rows at a time.
+struct Lanes {
+  int columns, row_threads;
+};
+
+// Bytes of scratch that joinRowThreads needs.
+__host__ __device__ constexpr size_t joinBytes(int vec, int threads) { return (size_t)threads * (vec > 2 ? vec : 2) * sizeof(float2); }
+
+// Each thread's two values (a, b) of each of its channels, joined over the block's row threads in double and in a fixed
+// order: value(row thread, values, row thread 0's values) is added up, and store(channel, sum, row thread 0's values)
+// called once for each of the block's channels.  The values lie side by side in `scratch`, so that lanes read and write
+// neighbouring words, and are added in two steps, `parts` threads to a channel first.
+template <int VEC, int THREADS, typename V, typename F>
+__device__ __forceinline__ void joinRowThreads(const Two (&a)[(VEC + 1) / 2], const Two (&b)[(VEC + 1) / 2], Lanes l,
+                                               float2 *scratch, V value, F store) {
+  const int tid = threadIdx.x, used = l.columns * l.row_threads;
+  __syncthreads();
+  if (tid < used) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float2 x = split(a[j / 2]), y = split(b[j / 2]);
+      scratch[j * used + tid] = j % 2 ? make_float2(x.y, y.y) : make_float2(x.x, y.x);
+    }
+  }
+  __syncthreads();
+  const int items = VEC * l.columns;  // (j, column), column fastest
+  int parts = THREADS / items;
+  parts = parts < 1 ? 1 : (parts > l.row_threads ? l.row_threads : parts);
+  auto add = [&](double2 &s, int row, float2 v, float2 v0) {
+    const double2 t = value(row, v, v0);
+    s.x += t.x;
+    s.y += t.y;
+  };
+  if (parts == 1) {
+    for (int item = tid; item < items; item += THREADS) {
+      const int column = item % l.columns, j = item / l.columns;
+      const float2 *from = scratch + j * used + column, v0 = from[0];
+      double2 s = make_double2(0.0, 0.0);
+      for (int row = 0; row < l.row_threads; ++row) add(s, row, from[row * l.columns], v0);
+      store(column * VEC + j, s, v0);
+    }
+    return;
+  }
+  double2 *joined = reinterpret_cast<double2 *>(scratch);  // (j, part, column) after the first step
+  double2 s = make_double2(0.0, 0.0);
+  const int column = tid % l.columns, part = tid / l.columns % parts, j = tid / (l.columns * parts);
+  if (j < VEC) {
+    const float2 *from = scratch + j * used + column, v0 = from[0];
+    for (int row = part; row < l.row_threads; row += parts) add(s, row, from[row * l.columns], v0);
+  }
+  const bool mine = tid < items;
+  const int own_column = tid % l.columns, own_j = tid / l.columns;
+  const float2 v0 = mine ? scratch[own_j * used + own_column] : make_float2(0.0f, 0.0f);
+  __syncthreads();
+  if (j < VEC) joined[tid] = s;
+  __syncthreads();
+  if (mine) {
+    s = make_double2(0.0, 0.0);
+    for (int k = 0; k < parts; ++k) {
+      const double2 v = joined[(own_j * parts + k) * l.columns + own_column];
+      s.x += v.x;
+      s.y += v.y;
+    }
+    store(own_column * VEC + own_j, s, v0);
+  }
+}
+struct PlainSums {
+  __device__ __forceinline__ double2 operator()(int, float2 v, float2) const { return make_double2(v.x, v.y); }
+};
+
+// (mean, sum of squared deviations) of each of a thread's channels over its `n` rows from sums about k.  Each thread takes
+// its own first row as k: the squares then lose no more than a factor of its few rows, wherever an outlier lies.
+template <int VEC>
+__device__ __forceinline__ void closeMoments(Two (&a)[(VEC + 1) / 2], Two (&b)[(VEC + 1) / 2],
+                                             const Two (&minus_k)[(VEC + 1) / 2], int n) {
+  const float over = n > 0 ? 1.0f / (float)n : 0.0f;
+  const Two inverse = two(over, over), minus = two(-1.0f, -1.0f);
+#pragma unroll
+  for (int j = 0; j < (VEC + 1) / 2; ++j) {
+    const Two off = a[j] * inverse;
+    const float2 squares = split(fma(a[j] * minus, off, b[j]));
+    b[j] = two(squares.x < 0.0f ? 0.0f : squares.x, squares.y < 0.0f ? 0.0f : squares.y);  // (NaN stays)
+    a[j] = off + minus_k[j] * minus;
+  }
+}
+// Joins them over the row threads of `rows` rows: store(channel, mean, sum of squared deviations).
+template <int VEC, int THREADS, typename F>
+__device__ __forceinline__ void joinMoments(const Two (&a)[(VEC + 1) / 2], const Two (&b)[(VEC + 1) / 2], Lanes l, int64_t rows,
+                                            float2 *scratch, F store) {
+  joinRowThreads<VEC, THREADS>(
+      a, b, l, scratch,
+      [&](int row, float2 v, float2 v0) {
+        const int64_t left = rows - row;
+        const double n = left > 0 ? (double)((left + l.row_threads - 1) / l.row_threads) : 0.0;
+        const double off = n > 0.0 ? (double)v.x - v0.x : 0.0;
+        return make_double2(n * off, n > 0.0 ? v.y + n * off * off : 0.0);
+      },
+      [&](int c, double2 s, float2 v0) {
+        const double off = s.x / (double)rows, squares = s.y - s.x * off;
+        store(c, v0.x + off, squares < 0.0 ? 0.0 : squares);
+      });
+}
+
 }  // namespace group_norm_act
 }  // namespace mluop
 

@@ -17,14 +17,15 @@
 // sums for sample s go to slot block + s, which is unique and makes the slots of one
 // sample neighbours, whatever the samples' sizes (they are known on the device only).
 //
-// Few rows: the three launches would take longer than their work.  There one block takes a
-// slice of channels that holds whole groups (forward: of one sample; backward: of all
-// samples one after the other, so that the affine gradients stay in the block) and does
-// all three steps; the second reading comes from L1 or L2.
+// Few rows in a sample: the three launches would take longer than their work, and many samples
+// would close a block's sums again and again.  There one block takes a slice of channels that
+// holds whole groups, of one sample (backward: of some samples one after the other) and does
+// all three steps; the second reading comes from L1 or L2.  Very few rows: a few lanes take a
+// (sample, group) (shortSamplesKernel).
 //
-// Variance: pass 1 sums x - k and (x - k)^2 with k the block's first value of that
-// channel, which is within a few deviations of the mean; the blocks' (mean, sum of
-// squared deviations) pairs are joined without cancellation.
+// Variance: pass 1 sums x - k and (x - k)^2 with k the thread's first value of that
+// channel; the threads' and the blocks' (mean, sum of squared deviations) pairs are
+// joined without cancellation.
 #include "kernels/group_norm_act/group_norm_act_kernels.h"
 
 #include <cuda_runtime.h>
@@ -46,68 +47,6 @@ constexpr int kThreads = 256;
 constexpr int kUnroll = 4;  // rows a thread has in flight
 constexpr int kSmallThreads = 512;
 constexpr int kSmallTurns = 16;  // rows a thread of the one-launch form takes, at most
-
-// A block's threads: `columns` side by side on a row, `row_threads` rows at a time.
-struct Lanes {
-  int columns, row_threads;
-};
-
-// Bytes of scratch that joinRowThreads needs.
-__host__ __device__ constexpr size_t joinBytes(int vec, int threads) { return (size_t)threads * (vec > 2 ? vec : 2) * sizeof(float2); }
-
-// A thread's sums (a, b) of each of its channels, added over the block's row threads in double and in a fixed order;
-// store(channel, sums) is called once for each of the block's channels.  The values lie side by side in `scratch`, so
-// that lanes read and write neighbouring words, and are added in two steps, `parts` threads to a channel first.
-template <int VEC, int THREADS, typename F>
-__device__ __forceinline__ void joinRowThreads(const Two (&a)[(VEC + 1) / 2], const Two (&b)[(VEC + 1) / 2], Lanes l,
-                                               float2 *scratch, F store) {
-  const int tid = threadIdx.x, used = l.columns * l.row_threads;
-  __syncthreads();
-  if (tid < used) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float2 x = split(a[j / 2]), y = split(b[j / 2]);
-      scratch[j * used + tid] = j % 2 ? make_float2(x.y, y.y) : make_float2(x.x, y.x);
-    }
-  }
-  __syncthreads();
-  const int items = VEC * l.columns;  // (j, column), column fastest
-  int parts = THREADS / items;
-  parts = parts < 1 ? 1 : (parts > l.row_threads ? l.row_threads : parts);
-  double2 *joined = reinterpret_cast<double2 *>(scratch);  // (j, part, column) after the first step
-  if (parts > 1) {
-    double2 s = make_double2(0.0, 0.0);
-    const int column = tid % l.columns, part = tid / l.columns % parts, j = tid / (l.columns * parts);
-    if (j < VEC) {
-      for (int row = part; row < l.row_threads; row += parts) {
-        const float2 v = scratch[j * used + row * l.columns + column];
-        s.x += v.x;
-        s.y += v.y;
-      }
-    }
-    __syncthreads();
-    if (j < VEC) joined[tid] = s;
-    __syncthreads();
-  }
-  for (int item = tid; item < items; item += THREADS) {
-    const int column = item % l.columns, j = item / l.columns;
-    double2 s = make_double2(0.0, 0.0);
-    if (parts > 1) {
-      for (int part = 0; part < parts; ++part) {
-        const double2 v = joined[(j * parts + part) * l.columns + column];
-        s.x += v.x;
-        s.y += v.y;
-      }
-    } else {
-      for (int row = 0; row < l.row_threads; ++row) {
-        const float2 v = scratch[j * used + row * l.columns + column];
-        s.x += v.x;
-        s.y += v.y;
-      }
-    }
-    store(column * VEC + j, s);
-  }
-}
 
 // Calls body(first row, last row + 1, sample) for the parts of rows begin .. end-1 that belong to one sample each, and
 // rest(first row) for the rows of no sample; by the whole block.
@@ -144,9 +83,10 @@ statisticsKernel(const T *x, Rows r, int channels, Lanes l, float2 *partial) {
     Two a[kPairs], b[kPairs], minus_k[kPairs];
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) a[j] = b[j] = minus_k[j] = two(0.0f, 0.0f);
-    if (active) {
+    const int own = active && stop - at > row ? (int)((stop - at - row + l.row_threads - 1) / l.row_threads) : 0;
+    if (own > 0) {
       Values<T, VEC> k;
-      k.load(x + at * channels + first);
+      k.load(x + (at + row) * channels + first);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) minus_k[j] = k.pair(j) * two(-1.0f, -1.0f);
       auto add = [&](const Values<T, VEC> &v) {
@@ -172,12 +112,10 @@ statisticsKernel(const T *x, Rows r, int channels, Lanes l, float2 *partial) {
         add(v);
       }
     }
-    const double n = (double)(stop - at);
+    closeMoments<VEC>(a, b, minus_k, own);
     float2 *out = partial + (blockIdx.x + sample) * channels + first0;
-    joinRowThreads<VEC, kThreads>(a, b, l, scratch, [&](int c, double2 s) {
-      if (first0 + c >= channels) return;
-      const double off = s.x / n, squares = s.y - s.x * off;
-      out[c] = make_float2((float)(toFloat(x[at * channels + first0 + c]) + off), squares < 0.0 ? 0.0f : (float)squares);
+    joinMoments<VEC, kThreads>(a, b, l, stop - at, scratch, [&](int c, double m, double squares) {
+      if (first0 + c < channels) out[c] = make_float2((float)m, (float)squares);
     });
   }, [](int64_t) {});
 }
@@ -351,7 +289,7 @@ gradSumsKernel(const T *dy, const T *x, const void *weight, const void *bias, bo
       }
     }
     float2 *out = partial + (blockIdx.x + sample) * channels + first0;
-    joinRowThreads<VEC, kThreads>(a, b, l, scratch, [&](int c, double2 s) {
+    joinRowThreads<VEC, kThreads>(a, b, l, scratch, PlainSums{}, [&](int c, double2 s, float2) {
       if (first0 + c < channels) out[c] = make_float2((float)s.x, (float)s.y);
     });
   }, [](int64_t) {});
@@ -484,12 +422,14 @@ inputGradKernel(const T *dy, const T *x, const void *weight, const void *bias, b
   });
 }
 
-// All three steps in one block: the slice of l.columns vectors from column blockIdx.x * l.columns on.
+// All three steps in one block: the slice of l.columns vectors from column blockIdx.y * l.columns on, of `chunk` samples
+// one after the other.  Backward, `partial` (more chunks than one): a line of the affine gradients' sums for each chunk.
 template <typename T, int VEC, int ACT, bool UNIFORM, bool BACKWARD>
 __global__ void __launch_bounds__(kSmallThreads, 1)
 sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool float_affine, float *mean, float *rstd,
-            Rows r, int channels, int groups, Lanes l, float epsilon, T *out, void *weight_grad, void *bias_grad,
-            bool float_affine_grad) {
+            Rows r, int channels, int groups, Lanes l, int64_t chunk, float epsilon, T *out, float2 *partial,
+            void *weight_grad, void *bias_grad, bool float_affine_grad) {
+  if (BACKWARD) letNextKernelStart();
   constexpr int kPairs = (VEC + 1) / 2, kGroups = UNIFORM ? 1 : kPairs;
   // joinRowThreads' scratch | the slice's channels (two doubles each) | its groups (two floats)
   extern __shared__ __align__(16) float2 scratch[];
@@ -497,12 +437,12 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
   double2 *sums = reinterpret_cast<double2 *>(scratch + joinBytes(VEC, kSmallThreads) / sizeof(float2));
   float2 *stats = reinterpret_cast<float2 *>(sums + slice);
   const int tid = threadIdx.x, row = tid / l.columns;
-  const int first0 = blockIdx.x * slice, own = tid % l.columns * VEC, first = first0 + own;
+  const int first0 = blockIdx.y * slice, own = tid % l.columns * VEC, first = first0 + own;
   const int group0 = first0 / group_channels;
   const bool active = row < l.row_threads;
   const int64_t step = (int64_t)l.row_threads * channels;
   double total_a = 0.0, total_b = 0.0;  // backward: thread c < slice adds up channel c over the samples
-  const int64_t s0 = BACKWARD ? 0 : blockIdx.y, s1 = BACKWARD ? r.samples : s0 + 1;
+  const int64_t s0 = blockIdx.x * chunk, s1 = s0 + chunk < r.samples ? s0 + chunk : r.samples;
   for (int64_t sample = s0; sample < s1; ++sample) {
     const int64_t begin = sampleStart(r, sample), end = sampleStart(r, sample + 1);
     const int rows = end > begin ? (int)(end - begin) : 0;
@@ -515,9 +455,9 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
     if (active && rows > 0) {
       if (BACKWARD) {
         loadNorm<T>(c, mean + sample * groups, rstd + sample * groups, weight, bias, float_affine, first, group_channels, r.one);
-      } else {
+      } else if (row < rows) {
         Values<T, VEC> k;
-        k.load(x + begin * channels + first);
+        k.load(from0);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) minus_k[j] = k.pair(j) * two(-1.0f, -1.0f);
       }
@@ -542,7 +482,12 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
         }
       }
     }
-    joinRowThreads<VEC, kSmallThreads>(a, b, l, scratch, [&](int ch, double2 v) { sums[ch] = v; });
+    if (BACKWARD) {
+      joinRowThreads<VEC, kSmallThreads>(a, b, l, scratch, PlainSums{}, [&](int ch, double2 v, float2) { sums[ch] = v; });
+    } else if (rows > 0) {
+      closeMoments<VEC>(a, b, minus_k, row < rows ? (rows - row + l.row_threads - 1) / l.row_threads : 0);
+      joinMoments<VEC, kSmallThreads>(a, b, l, rows, scratch, [&](int ch, double m, double squares) { sums[ch] = make_double2(m, squares); });
+    }
     __syncthreads();
     if (BACKWARD) {
       if (tid < slice) {  // (slice <= kSmallThreads)
@@ -559,12 +504,10 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
           const double gamma = weight ? (double)loadAffine<T>(weight, float_affine, first0 + ch) : 1.0;
           u += gamma * v.x;
           w += gamma * v.y;
-        } else if (rows > 0) {  // (sum, squares) about the channel's first value
-          const double off = v.x / rows, m = (double)toFloat(x[begin * channels + first0 + ch]) + off;
-          if (i == 0) ref = m;
-          const double squares = v.y - v.x * off;
-          u += m - ref;
-          w += (squares < 0.0 ? 0.0 : squares) + rows * (m - ref) * (m - ref);  // (NaN stays)
+        } else if (rows > 0) {
+          if (i == 0) ref = v.x;
+          u += v.x - ref;
+          w += v.y + rows * (v.x - ref) * (v.x - ref);
         }
       }
       const double n = (double)(rows > 0 ? rows : 1) * group_channels;
@@ -629,12 +572,45 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
     }
   }
   if (BACKWARD && weight_grad && tid < slice) {
-    storeAffineGrad<T>(bias_grad, float_affine_grad, first0 + tid, total_a);
-    storeAffineGrad<T>(weight_grad, float_affine_grad, first0 + tid, total_b);
+    if (partial) {
+      partial[(int64_t)blockIdx.x * channels + first0 + tid] = make_float2((float)total_a, (float)total_b);
+    } else {
+      storeAffineGrad<T>(bias_grad, float_affine_grad, first0 + tid, total_a);
+      storeAffineGrad<T>(weight_grad, float_affine_grad, first0 + tid, total_b);
+    }
   }
-  if (active && (BACKWARD || blockIdx.y == 0)) {  // rows of no sample
+  if (active && blockIdx.x == 0) {  // rows of no sample
     const int64_t covered = sampleStart(r, r.samples);
     for (int64_t i = covered + row; i < r.rows; i += l.row_threads) Values<T, VEC>::storeZero(out + i * channels + first);
+  }
+}
+
+// The affine gradients as sums over `lines` lines of (sum du, sum du xhat) per channel, in a fixed order: 32 channels
+// side by side in a block, 32 threads along the lines.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+affineGradKernel(const float2 *sums, int64_t lines, int channels, void *weight_grad, void *bias_grad, bool float_affine_grad) {
+  __shared__ double2 part[32][33];
+  const int c = threadIdx.x % 32, d = threadIdx.x / 32, channel = blockIdx.x * 32 + c;
+  double a = 0.0, b = 0.0;
+  waitForKernelBefore();
+  if (channel < channels) {
+#pragma unroll 4
+    for (int64_t k = d; k < lines; k += 32) {
+      const float2 v = sums[k * channels + channel];
+      a += v.x;
+      b += v.y;
+    }
+  }
+  part[d][c] = make_double2(a, b);
+  __syncthreads();
+  if (d == 0 && channel < channels) {
+    for (int i = 1; i < 32; ++i) {
+      a += part[i][c].x;
+      b += part[i][c].y;
+    }
+    storeAffineGrad<T>(bias_grad, float_affine_grad, channel, a);
+    storeAffineGrad<T>(weight_grad, float_affine_grad, channel, b);
   }
 }
 
@@ -654,39 +630,68 @@ double rowBytes(const NormProblem &p) {
 
 }  // namespace
 
-// Measured on 256 x 128 values of 2 samples: one launch 6 us against 15 us for the three.
-int sliceColumns(const NormProblem &p, int vec, bool backward) {
-  if (p.samples == 0) return 0;
-  const int group_channels = p.channels / p.groups;
-  const int columns = std::lcm(group_channels, vec) / vec;
-  if (columns * vec > kSmallThreads || p.channels % (columns * vec) != 0) return 0;
-  // rows of one block: backward all of them; forward a sample's (on average) and, of the rows of no sample, all there may be
-  const int64_t rows = backward ? p.rows : (p.rows + p.samples - 1) / p.samples;
-  const int64_t turns = kSmallThreads / columns * (int64_t)kSmallTurns;
-  if (rows > turns || p.rows > 16 * turns || p.samples > (backward ? 64 : 65535)) return 0;
-  return columns;
-}
-
 namespace {
 
+constexpr int kAffineSamples = 32;  // more: their sums are added up by a kernel of its own
+
+// The one-launch form for samples of few rows: slices of `columns` vectors, `chunk` samples a block.  columns 0: it does
+// not apply.  Measured on 256 x 128 values of 2 samples: one launch 6 us against 15 us for the three.
+struct SlicePlan {
+  int columns;
+  int64_t chunk, chunks;
+};
+SlicePlan planSlices(const NormProblem &p, int vec, bool backward) {
+  SlicePlan plan{};
+  if (p.samples == 0) return plan;
+  const int group_channels = p.channels / p.groups;
+  const int columns = std::lcm(group_channels, vec) / vec;
+  if (columns * vec > kSmallThreads || p.channels % (columns * vec) != 0 || p.channels / (columns * vec) > 65535) return plan;
+  // rows of one sample: where they are known on the device only, their average, and few in all, since one sample may have
+  // them all
+  const int64_t rows = p.ragged ? (p.rows + p.samples - 1) / p.samples : p.sample_rows;
+  const int64_t turns = kSmallThreads / columns * (int64_t)kSmallTurns;
+  if (rows > turns || (p.ragged && p.rows > 16 * turns)) return plan;
+  // one round of blocks: 2,048 blocks for 256 samples of 64 rows of 128 channels took 74 us against 19 us for the three
+  const int64_t slices = p.channels / (columns * vec), most = std::max<int64_t>(1, 2 * p.sm_count / slices);
+  if (p.samples > most || (!p.ragged && rows <= kShortRows)) return plan;
+  plan.columns = columns;
+  plan.chunk = backward && p.samples <= 4 ? p.samples : 1;  // backward, up to four: in one block, which writes the affine gradients
+  plan.chunks = (p.samples + plan.chunk - 1) / plan.chunk;
+  return plan;
+}
+
+template <typename T>
+cudaError_t launchAffineGrad(const NormProblem &p, const float2 *sums, int64_t lines, void *weight_grad, void *bias_grad,
+                             cudaStream_t stream) {
+  trace::Scope scope("groupNormAffineGradKernel", stream);
+  return launchAfterKernel(affineGradKernel<T>, dim3((unsigned)((p.channels + 31) / 32)), dim3(1024), 0, stream, sums, lines,
+                           p.channels, weight_grad, bias_grad, p.float_affine_grad);
+}
+
 template <typename T, int VEC, bool UNIFORM, bool BACKWARD>
-cudaError_t launchSlices(const NormProblem &p, int columns, const void *output_grad, const void *input, const void *weight,
-                         const void *bias, float *mean, float *rstd, void *out, void *weight_grad, void *bias_grad,
-                         cudaStream_t stream) {
-  const Lanes l{columns, kSmallThreads / columns};
-  const int slice = columns * VEC;
+cudaError_t launchSlices(const NormProblem &p, const SlicePlan &plan, const void *output_grad, const void *input,
+                         const void *weight, const void *bias, void *workspace, float *mean, float *rstd, void *out,
+                         void *weight_grad, void *bias_grad, cudaStream_t stream) {
+  const Lanes l{plan.columns, kSmallThreads / plan.columns};
+  const int slice = plan.columns * VEC;
   const size_t smem = joinBytes(VEC, kSmallThreads) + slice * sizeof(double2) + slice / (p.channels / p.groups) * sizeof(float2);
-  const dim3 grid((unsigned)(p.channels / slice), BACKWARD ? 1u : (unsigned)p.samples);
-  trace::Scope scope(BACKWARD ? "groupNormSliceKernel:backward" : "groupNormSliceKernel:forward", stream,
-                     (BACKWARD ? 3 : 2) * rowBytes(p));
+  const dim3 grid((unsigned)plan.chunks, (unsigned)(p.channels / slice));
+  float2 *partial = BACKWARD && weight_grad && plan.chunks > 1 ? reinterpret_cast<float2 *>(scratchBase(workspace)) : nullptr;
   auto kernel = p.activation == MLUOP_GROUP_NORM_ACT_RELU   ? sliceKernel<T, VEC, MLUOP_GROUP_NORM_ACT_RELU, UNIFORM, BACKWARD>
                 : p.activation == MLUOP_GROUP_NORM_ACT_SILU ? sliceKernel<T, VEC, MLUOP_GROUP_NORM_ACT_SILU, UNIFORM, BACKWARD>
                                                             : sliceKernel<T, VEC, MLUOP_GROUP_NORM_ACT_NONE, UNIFORM, BACKWARD>;
   const Rows r{p.rows, p.samples, p.sample_rows, 0, p.sample_ends, 1.0f};
-  kernel<<<grid, kSmallThreads, smem, stream>>>(static_cast<const T *>(output_grad), static_cast<const T *>(input), weight,
-                                                bias, p.float_affine, mean, rstd, r, p.channels, p.groups, l, p.epsilon,
-                                                static_cast<T *>(out), weight_grad, bias_grad, p.float_affine_grad);
-  return cudaGetLastError();
+  {
+    trace::Scope scope(BACKWARD ? "groupNormSliceKernel:backward" : "groupNormSliceKernel:forward", stream,
+                       (BACKWARD ? 3 : 2) * rowBytes(p));
+    kernel<<<grid, kSmallThreads, smem, stream>>>(static_cast<const T *>(output_grad), static_cast<const T *>(input), weight,
+                                                  bias, p.float_affine, mean, rstd, r, p.channels, p.groups, l, plan.chunk,
+                                                  p.epsilon, static_cast<T *>(out), partial, weight_grad, bias_grad,
+                                                  p.float_affine_grad);
+  }
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess || !partial) return err;
+  return launchAffineGrad<T>(p, partial, plan.chunks, weight_grad, bias_grad, stream);
 }
 
 template <typename T, int VEC, bool UNIFORM>
@@ -746,10 +751,17 @@ cudaError_t backward(const NormProblem &p, const NormPlan &plan, const void *out
                             weight, p.float_affine, r, p.channels, p.groups, sample_sums, group_means);
   }
   if (err != cudaSuccess) return err;
-  trace::Scope scope("groupNormInputGradKernel", stream, 3 * rowBytes(p));
-  return launchAfterKernel(inputGradKernel<T, VEC, ACT, UNIFORM>, grid, dim3(kThreads), 0, stream, dy, x, weight, bias,
-                           p.float_affine, mean, rstd, sample_sums, group_means, r, p.channels, p.groups, l,
-                           static_cast<T *>(input_grad), weight_grad, bias_grad, p.float_affine_grad);
+  const bool many = weight_grad && p.samples > kAffineSamples;
+  {
+    trace::Scope scope("groupNormInputGradKernel", stream, 3 * rowBytes(p));
+    void *none = nullptr;
+    err = launchAfterKernel(inputGradKernel<T, VEC, ACT, UNIFORM>, grid, dim3(kThreads), 0, stream, dy, x, weight, bias,
+                            p.float_affine, mean, rstd, sample_sums, group_means, r, p.channels, p.groups, l,
+                            static_cast<T *>(input_grad), many ? none : weight_grad, many ? none : bias_grad,
+                            p.float_affine_grad);
+  }
+  if (err != cudaSuccess || !many) return err;
+  return launchAffineGrad<T>(p, sample_sums, p.samples, weight_grad, bias_grad, stream);
 }
 
 template <typename T, int VEC, bool UNIFORM, typename... Args>
@@ -801,10 +813,16 @@ NormPlan planNorm(const NormProblem &p, bool backward, bool vectors) {
 }
 
 size_t normWorkspaceBytes(const NormProblem &p, bool backward) {
-  // whichever way the tensors are aligned, the one-launch form needs none
+  // whichever way the tensors are aligned
+  auto bytes = [&](int vec) -> size_t {
+    if (const SlicePlan plan = planSlices(p, vec, backward); plan.columns)
+      return backward && plan.chunks > 1 ? (size_t)plan.chunks * p.channels * sizeof(float2) + 256 : 0;
+    if (const ShortPlan plan = planShort(p, vec); plan.lanes)
+      return backward ? (size_t)plan.blocks * p.channels * sizeof(float2) + 256 : 0;
+    return planNorm(p, backward, vec > 1).total;
+  };
   const int wide = 16 / (int)mluop::getSizeOfDataType(p.dtype);
-  if (sliceColumns(p, 1, backward) && (p.channels % wide != 0 || sliceColumns(p, wide, backward))) return 0;
-  return std::max(planNorm(p, backward, true).total, planNorm(p, backward, false).total);
+  return p.channels % wide != 0 ? bytes(1) : std::max(bytes(1), bytes(wide));
 }
 
 namespace {
@@ -813,12 +831,14 @@ template <typename T, int VEC>
 cudaError_t runForward(const NormProblem &p, const void *input, const void *weight, const void *bias, void *workspace,
                        void *output, float *mean, float *rstd, cudaStream_t stream) {
   const NormPlan plan = planNorm(p, false, aligned16(input) && aligned16(output));
-  if (const int columns = sliceColumns(p, plan.vec, false)) {
+  if (const SlicePlan slices = planSlices(p, plan.vec, false); slices.columns) {
     auto launch = plan.vec == 1                        ? launchSlices<T, 1, true, false>
                   : p.channels / p.groups % VEC == 0 ? launchSlices<T, VEC, true, false>
                                                      : launchSlices<T, VEC, false, false>;
-    return launch(p, columns, nullptr, input, weight, bias, mean, rstd, output, nullptr, nullptr, stream);
+    return launch(p, slices, nullptr, input, weight, bias, workspace, mean, rstd, output, nullptr, nullptr, stream);
   }
+  if (const ShortPlan few = planShort(p, plan.vec); few.lanes)
+    return launchShortForward(p, few, input, weight, bias, output, mean, rstd, stream);
   return forwardType<T, VEC>(p, plan, input, weight, bias, workspace, output, mean, rstd, stream);
 }
 
@@ -827,12 +847,18 @@ cudaError_t runBackward(const NormProblem &p, const void *output_grad, const voi
                         const void *bias, const float *mean, const float *rstd, void *workspace, void *input_grad,
                         void *weight_grad, void *bias_grad, cudaStream_t stream) {
   const NormPlan plan = planNorm(p, true, aligned16(output_grad) && aligned16(input) && aligned16(input_grad));
-  if (const int columns = sliceColumns(p, plan.vec, true)) {
+  if (const SlicePlan slices = planSlices(p, plan.vec, true); slices.columns) {
     auto launch = plan.vec == 1                        ? launchSlices<T, 1, true, true>
                   : p.channels / p.groups % VEC == 0 ? launchSlices<T, VEC, true, true>
                                                      : launchSlices<T, VEC, false, true>;
-    return launch(p, columns, output_grad, input, weight, bias, const_cast<float *>(mean), const_cast<float *>(rstd),
+    return launch(p, slices, output_grad, input, weight, bias, workspace, const_cast<float *>(mean), const_cast<float *>(rstd),
                   input_grad, weight_grad, bias_grad, stream);
+  }
+  if (const ShortPlan few = planShort(p, plan.vec); few.lanes) {
+    float2 *partial = weight_grad ? reinterpret_cast<float2 *>(scratchBase(workspace)) : nullptr;
+    const cudaError_t err = launchShortBackward(p, few, output_grad, input, weight, bias, mean, rstd, partial, input_grad, stream);
+    return err != cudaSuccess || !partial ? err
+                                          : launchAffineGrad<T>(p, partial, few.blocks, weight_grad, bias_grad, stream);
   }
   return backwardType<T, VEC>(p, plan, output_grad, input, weight, bias, mean, rstd, workspace, input_grad, weight_grad,
                               bias_grad, stream);

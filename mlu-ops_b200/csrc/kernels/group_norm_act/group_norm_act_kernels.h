@@ -17,7 +17,8 @@ struct NormProblem {
   bool float_affine, float_affine_grad;  // weight and bias (and their gradients) in float, else in `dtype`
   int64_t rows;         // all rows
   int64_t samples;
-  int64_t sample_rows;  // rows of each sample where sample_ends is null
+  bool ragged;          // sample_ends is given
+  int64_t sample_rows;  // rows of each sample where it is not
   int channels, groups;
   const int32_t *sample_ends;
   float epsilon;
@@ -37,8 +38,26 @@ struct NormPlan {
   size_t partial, sample_sums, group_means, total;
 };
 
-// The one-launch form for few rows: the width of its slices in vectors of `vec` channels, or 0 where it does not apply.
-int sliceColumns(const NormProblem &p, int vec, bool backward);
+// The form for samples of very few rows (group_norm_act_short.cu).
+constexpr int kShortRows = 8;       // it takes samples of up to as many rows always,
+constexpr int kMostShortRows = 64;  // and of up to as many where there are enough samples
+struct ShortPlan {
+  int vec;            // channels of a vector
+  int lanes;          // of one (sample, group): a power of two, at most a warp; 0: the form does not apply
+  int vectors;        // of a lane, at most
+  int groups_block;   // groups side by side in a block
+  int samples_block;  // samples of a block at a time
+  int tiles;          // blocks along the groups
+  int64_t blocks;     // and along the samples
+};
+ShortPlan planShort(const NormProblem &p, int vec);
+cudaError_t launchShortForward(const NormProblem &p, const ShortPlan &plan, const void *input, const void *weight,
+                               const void *bias, void *output, float *mean, float *rstd, cudaStream_t stream);
+// partial: null, or the sums of du and du xhat, a line of `channels` for each of plan.blocks
+cudaError_t launchShortBackward(const NormProblem &p, const ShortPlan &plan, const void *output_grad, const void *input,
+                                const void *weight, const void *bias, const float *mean, const float *rstd, float2 *partial,
+                                void *input_grad, cudaStream_t stream);
+
 NormPlan planNorm(const NormProblem &p, bool backward, bool vectors);
 size_t normWorkspaceBytes(const NormProblem &p, bool backward);
 

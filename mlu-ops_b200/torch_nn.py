@@ -119,7 +119,8 @@ class AdamW(torch.optim.Optimizer):
     bfloat16; states are held in float or 8 bits whatever the parameter's type.  capturable=True keeps the
     step count and the learning rate of each parameter group on the device, so that a captured step can be
     replayed (lr may then be a CUDA tensor; one step count for the whole group).  step(grad_scale=t)
-    multiplies every gradient by the float32 CUDA tensor t of one element.
+    multiplies every gradient by the float32 CUDA tensor t of one element.  Before a step is captured, run one
+    outside of the capture: it allocates the states and the handles.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
@@ -155,6 +156,8 @@ class AdamW(torch.optim.Optimizer):
         at = [list(map(torch.Tensor.data_ptr, v)) for v in tensors]
         known = self._plans.get(key)
         if known is None or known[0] != at:
+            if len(self._plans) >= 64:  # the set of parameters that have gradients changes from step to step
+                self._plans.clear()
             known = self._plans[key] = (at, ops.MultiTensorAdamW(*tensors))
         return known[1]
 
@@ -204,6 +207,14 @@ class AdamW(torch.optim.Optimizer):
                           group["weight_decay"], max(count, 1), grad_scale=grad_scale, **more)
         return loss
 
+    def __getstate__(self):  # (copies and pickles; what is laid out for the calls is not part of it)
+        return {**super().__getstate__(), "state_bits": self.state_bits, "capturable": self.capturable,
+                "_schedules": self._schedules}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plans = {}
+
     def state_dict(self):
         out = super().state_dict()
         out["schedules"] = {i: (c.clone(), b.clone()) for i, (c, b) in self._schedules.items()}
@@ -214,6 +225,8 @@ class AdamW(torch.optim.Optimizer):
         them to the parameters')."""
         state_dict = dict(state_dict)
         schedules = state_dict.pop("schedules", {})
+        if any(("exp_avg_scale" in s) != (self.state_bits == 8) for s in state_dict["state"].values()):
+            raise ValueError("the saved states have another number of bits")
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]

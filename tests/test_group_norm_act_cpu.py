@@ -106,9 +106,26 @@ def test_backward_refuses(ops, handle, over):
 
 
 def test_few_rows_need_no_workspace(ops, handle):
-    c = Call(ops, handle, null=("ws",))
+    c = Call(ops, handle, dims=(2, 20, 16), null=("ws",))
     assert c.workspace(False) == (ops.STATUS_SUCCESS, 0) and c.workspace(True) == (ops.STATUS_SUCCESS, 0)
     assert c.forward() == ops.STATUS_EXECUTION_FAILED and c.backward() == ops.STATUS_EXECUTION_FAILED
+
+
+def test_in_place_or_apart(ops, handle):
+    size = 2 * 20 * 16 * 2
+    for shift, want in ((0, ops.STATUS_EXECUTION_FAILED), (16, ops.STATUS_BAD_PARAM), (-16, ops.STATUS_BAD_PARAM),
+                        (size, ops.STATUS_EXECUTION_FAILED), (size - 2, ops.STATUS_BAD_PARAM)):
+        for name in ("x", "dy"):
+            c = Call(ops, handle, dims=(2, 20, 16))
+            out = ("y", "dx") if name == "x" else ("dx",)
+            for o in out:
+                c.shift = {o: 4096 * (sorted(c.t).index(name) - sorted(c.t).index(o)) + shift}
+                assert (c.forward() if o == "y" else c.backward()) == want
+
+
+def test_epsilon_is_positive_in_float(ops, handle):
+    assert Call(ops, handle, eps=1e-50).forward() == ops.STATUS_BAD_PARAM
+    assert Call(ops, handle, eps=1e39).forward() == ops.STATUS_BAD_PARAM
 
 
 def test_null_handle_and_descriptors(ops, handle):

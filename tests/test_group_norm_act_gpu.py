@@ -3,7 +3,9 @@
 Tolerances, u = 2^-24 (half a step of float), sums of n values in float off by at most d u times
 the sum of magnitudes, d the number of additions that one value passes through: a thread adds at
 most 64 rows here and a block joins its threads in 8 levels: d = 72; the blocks' sums are joined in
-double.  Statistics: with k the block's first row, deviations from it average at most |x - k|, whose
+double.  (Short samples: a thread adds at most 64 rows of 4 pairs.  Deviations are from the group's mean as float sums give
+it, each rounded once: with A1 and A2 the group's mean deviation and variance, the mean and the variance are off by no more
+than the terms below, d = 4 * 64 + 1.)  Statistics: with k the block's first row, deviations from it average at most |x - k|, whose
 mean over a group is bounded by the test from the data (A1, and A2 for squares): the mean is off by
 d u A1 + 2 u |mean|, the variance by 2 d u A2 + 4 u A2.  xhat = (x - mean) rstd then by
 (d_mean + u |x| ) rstd + |xhat| (d_var / (2 var') + 4 u); y adds the two roundings of the affine
@@ -95,8 +97,12 @@ def check(ops, handle, shape, groups, dtype, act, ends=None, seed=0, affine="flo
         # the largest deviation from any row of the sample bounds the one from the block's first row
         spread = (r.amax(0) - r.amin(0))
         a1, a2 = spread.mean(1), (spread ** 2).mean(1)
-        d_mean = D * U * a1 + 4 * U * m.abs() + 1e-38
-        d_var = 2 * (D + 4) * U * a2
+        depth = D
+        if ends is None and hi - lo <= 64:
+            depth = 4 * (hi - lo) + 1
+            a1, a2 = (r - m[None, :, None]).abs().mean((0, 2)), var
+        d_mean = depth * U * a1 + 4 * U * m.abs() + 1e-38
+        d_var = 2 * (depth + 4) * U * a2
         within(mean[i], m, d_mean, "mean")
         want_r = (var + EPS) ** -0.5
         within(rstd[i], want_r, want_r * (d_var / (2 * (var + EPS)) + 4 * U) * 1.01, "rstd")
@@ -157,6 +163,54 @@ def test_maps(ops, gpu_handle, guard_bands, dtype, act):
 def test_shapes(ops, gpu_handle, guard_bands, shape, groups):
     check(ops, gpu_handle, shape, groups, torch.float32, "silu", seed=2)
     check(ops, gpu_handle, shape, groups, torch.float16, "relu", seed=3)
+
+
+@pytest.mark.parametrize("shape,groups", [((2, 8), 2), ((300, 64), 8), ((600, 2048), 32), ((513, 4096), 4096), ((70, 1, 128), 128),
+                                          ((33, 5, 48), 3), ((900, 3, 30), 10), ((5, 64, 256), 1), ((40, 2, 2048), 32),
+                                          ((9, 64, 64), 4), ((9, 65, 64), 4), ((50, 2, 3, 24), 2), ((200, 45), 1), ((3, 33), 1),
+                                          ((300, 512), 1), ((100, 3, 1024), 1), ((50, 2, 240), 2), ((30, 4, 1536), 1)])
+@pytest.mark.parametrize("dtype,act", [(torch.float32, "none"), (torch.float16, "silu"), (torch.bfloat16, "relu")])
+def test_short_samples(ops, gpu_handle, guard_bands, shape, groups, dtype, act):
+    """Up to 64 rows a sample; [N, C] is a sample a row."""
+    check(ops, gpu_handle, shape, groups, dtype, act, seed=21)
+
+
+@pytest.mark.parametrize("shape,groups", [((40, 100, 64), 8), ((700, 80, 32), 4), ((5, 200, 24), 3), ((300, 65, 512), 1), ((600, 1, 45), 1)])
+@pytest.mark.parametrize("dtype,act", [(torch.float32, "silu"), (torch.float16, "relu")])
+def test_many_samples_of_few_rows(ops, gpu_handle, guard_bands, shape, groups, dtype, act):
+    check(ops, gpu_handle, shape, groups, dtype, act, seed=23)
+
+
+def test_many_ragged_samples(ops, gpu_handle, guard_bands):
+    gen = torch.Generator().manual_seed(24)
+    ends = torch.randint(0, 60, (150,), generator=gen).cumsum(0).tolist()
+    check(ops, gpu_handle, (ends[-1] + 11, 32), 4, torch.float16, "silu", ends=ends, seed=25)
+    ends = torch.randint(300, 600, (70,), generator=gen).cumsum(0).tolist()
+    check(ops, gpu_handle, (ends[-1] + 11, 128), 8, torch.float32, "relu", ends=ends, seed=26)
+
+
+@pytest.mark.parametrize("shape,thread_rows", [((1, 4096, 128), 64), ((3, 50, 32), 1), ((8, 200000, 16), 44)])
+def test_an_outlier_in_the_first_row(ops, gpu_handle, shape, thread_rows):
+    """One value of 1e4 among values of size 1.  The thread that has it in its n rows sums up to n squares about it, n times
+    the sample's whole sum of squares, in n additions that round by half a step of what is there by then: n^2 / 2 half steps
+    of the variance, half of that for rstd, and four half steps for the rest."""
+    x, _, _, _ = make(shape, torch.float32, 27, affine=None)
+    x[:, 0] = 1e4
+    _, _, rstd = ops.group_norm_act_forward(gpu_handle, x, None, None, 4, EPS, "none")
+    var = x.double().reshape(shape[0], shape[1], 4, -1).var((1, 3), unbiased=False)
+    assert ((rstd.double() * (var + EPS).sqrt() - 1).abs() <= (thread_rows ** 2 / 4 + 4) * U).all()
+
+
+def test_short_samples_in_place_and_unaligned(ops, gpu_handle):
+    x, w, b, dy = make((700, 2, 64), torch.float16, 22)
+    raw = torch.zeros(x.numel() + 1, dtype=x.dtype, device="cuda")
+    off = raw[1:].view(x.shape).copy_(x)
+    y, mean, rstd = ops.group_norm_act_forward(gpu_handle, x, w, b, 8, EPS, "silu")
+    y1, mean1, rstd1 = ops.group_norm_act_forward(gpu_handle, off, w, b, 8, EPS, "silu", out=off)
+    assert torch.allclose(y, y1, atol=2e-3) and torch.allclose(rstd, rstd1, rtol=1e-5)
+    want = ops.group_norm_act_backward(gpu_handle, dy, x, w, b, mean, rstd, 8, "silu")
+    got = ops.group_norm_act_backward(gpu_handle, dy, x, w, b, mean, rstd, 8, "silu", out=dy)
+    assert got[0] is dy and all(torch.equal(p, q) for p, q in zip(want, got))
 
 
 @pytest.mark.parametrize("rows,ends", [(1000, [300, 301, 301, 900]), (700, [0, 0, 700]), (513, [513]), (90, [0]), (50, [50, 50, 50]),

@@ -16,6 +16,8 @@ def handle(ops):
 
 
 class Call:
+    APART = 1 << 22  # between the tensors' addresses, which nothing reads
+
     def __init__(self, ops, handle, dtype=HALF, rows=10, groups=3, ci=16, co=24, **over):
         self.ops, self.handle = ops, handle
         self.t = dict(x=(dtype, (rows, ci)), y=(dtype, (rows, co)), w=(dtype, (groups, ci, co)), e=(I32, (groups,)))
@@ -28,7 +30,7 @@ class Call:
     def ptr(self, name):
         if name in self.null or self.d.get(name, 0) is None:
             return None
-        return ctypes.c_void_p(self.base + 4096 * "xywes".index(name) + self.shift.get(name, 0))
+        return ctypes.c_void_p(self.base + self.APART * "xywes".index(name) + self.shift.get(name, 0))
 
     def pairs(self, *names):
         return [a for n in names for a in (self.d[n], self.ptr(n))]
@@ -65,6 +67,16 @@ def test_valid_calls_reach_the_launch(ops, handle, over):
 def test_float_weight_gradient(ops, handle):
     c = Call(ops, handle, w=(FLOAT, (3, 16, 24)))
     assert c.all() == [ops.STATUS_BAD_PARAM, ops.STATUS_BAD_PARAM, ops.STATUS_EXECUTION_FAILED]
+
+
+def test_outputs_lie_on_no_input(ops, handle):
+    at = "xywes".index
+    for out, call, inputs in (("y", "forward", "xwe"), ("x", "backward_input", "ywe"), ("w", "backward_weight", "xye")):
+        for name in inputs:
+            for off in (0, 4):
+                c = Call(ops, handle)
+                c.shift = {out: c.APART * (at(name) - at(out)) + off}
+                assert getattr(c, call)() == ops.STATUS_BAD_PARAM
 
 
 def test_no_rows(ops, handle):

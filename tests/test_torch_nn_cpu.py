@@ -37,3 +37,25 @@ def test_modules_hold_their_parameters(nn_):
     g = nn_.GroupNormAct(4, 16)
     assert (g.weight == 1).all() and not g.bias.any()
     assert nn_.GroupNormAct(4, 16, affine=False).weight is None
+
+
+def test_optimizer_copies_and_pickles(nn_):
+    import copy
+    import pickle
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = nn_.AdamW([p], lr=1e-2, state_bits=8, capturable=True)
+    opt._plans[0] = lambda: None  # what is laid out for the calls stays behind
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.state_bits == 8 and other.capturable and other._plans == {} and other._schedules == {}
+        assert other.param_groups[0]["lr"] == 1e-2 and other.param_groups[0]["params"][0] is not p
+
+
+def test_optimizer_refuses_states_of_other_bits(nn_):
+    p = torch.nn.Parameter(torch.zeros(4))
+    saved = {bits: nn_.AdamW([p], state_bits=bits) for bits in (8, 32)}
+    for opt in saved.values():
+        opt.state[p] = opt._new_state(p)
+    for bits in (8, 32):
+        nn_.AdamW([p], state_bits=bits).load_state_dict(saved[bits].state_dict())
+        with pytest.raises(ValueError):
+            nn_.AdamW([p], state_bits=bits).load_state_dict(saved[40 - bits].state_dict())
