@@ -206,15 +206,16 @@ __device__ __forceinline__ void closeMoments(Two (&a)[(VEC + 1) / 2], Two (&b)[(
 }
 // Joins them over the row threads of `rows` rows: store(channel, mean, sum of squared deviations).
 template <int VEC, int THREADS, typename F>
-__device__ __forceinline__ void joinMoments(const Two (&a)[(VEC + 1) / 2], const Two (&b)[(VEC + 1) / 2], Lanes l, int64_t rows,
+__device__ __forceinline__ void joinMoments(const Two (&a)[(VEC + 1) / 2], const Two (&b)[(VEC + 1) / 2], Lanes l, int rows,
                                             float2 *scratch, F store) {
+  const int each = rows / l.row_threads, more = rows % l.row_threads;  // rows of a thread, threads with one more
   joinRowThreads<VEC, THREADS>(
       a, b, l, scratch,
       [&](int row, float2 v, float2 v0) {
-        const int64_t left = rows - row;
-        const double n = left > 0 ? (double)((left + l.row_threads - 1) / l.row_threads) : 0.0;
-        const double off = n > 0.0 ? (double)v.x - v0.x : 0.0;
-        return make_double2(n * off, n > 0.0 ? v.y + n * off * off : 0.0);
+        const int own = each + (row < more);
+        if (own == 0) return make_double2(0.0, 0.0);
+        const double off = (double)v.x - v0.x, part = own * off;
+        return make_double2(part, v.y + part * off);
       },
       [&](int c, double2 s, float2 v0) {
         const double off = s.x / (double)rows, squares = s.y - s.x * off;

@@ -46,7 +46,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;  // rows a thread has in flight
 constexpr int kSmallThreads = 512;
-constexpr int kSmallTurns = 16;  // rows a thread of the one-launch form takes, at most
+constexpr int kSmallTurns = 4;   // rows a thread of the one-launch form takes, at most
 
 // Calls body(first row, last row + 1, sample) for the parts of rows begin .. end-1 that belong to one sample each, and
 // rest(first row) for the rows of no sample; by the whole block.
@@ -83,7 +83,7 @@ statisticsKernel(const T *x, Rows r, int channels, Lanes l, float2 *partial) {
     Two a[kPairs], b[kPairs], minus_k[kPairs];
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) a[j] = b[j] = minus_k[j] = two(0.0f, 0.0f);
-    const int own = active && stop - at > row ? (int)((stop - at - row + l.row_threads - 1) / l.row_threads) : 0;
+    const int own = active && stop - at > row ? ((int)(stop - at) - row + l.row_threads - 1) / l.row_threads : 0;
     if (own > 0) {
       Values<T, VEC> k;
       k.load(x + (at + row) * channels + first);
@@ -114,7 +114,7 @@ statisticsKernel(const T *x, Rows r, int channels, Lanes l, float2 *partial) {
     }
     closeMoments<VEC>(a, b, minus_k, own);
     float2 *out = partial + (blockIdx.x + sample) * channels + first0;
-    joinMoments<VEC, kThreads>(a, b, l, stop - at, scratch, [&](int c, double m, double squares) {
+    joinMoments<VEC, kThreads>(a, b, l, (int)(stop - at), scratch, [&](int c, double m, double squares) {
       if (first0 + c < channels) out[c] = make_float2((float)m, (float)squares);
     });
   }, [](int64_t) {});
@@ -635,7 +635,10 @@ namespace {
 constexpr int kAffineSamples = 32;  // more: their sums are added up by a kernel of its own
 
 // The one-launch form for samples of few rows: slices of `columns` vectors, `chunk` samples a block.  columns 0: it does
-// not apply.  Measured on 256 x 128 values of 2 samples: one launch 6 us against 15 us for the three.
+// not apply.  Its blocks read 32 bytes or so of a row, and the chained launches of the other form cost about 9 us together.
+// Measured, half, forward and gradients: 2 samples of 128 rows of 128 channels 6.5 and 9.4 us against 9.5 and 9.9 us, 8 of
+// 1,024 rows of 256 channels 9.5 and 11 us against 13.5 and 14 us, 2 of 2,048 rows of 128 channels 12 and 24 us against 10
+// and 10 us.
 struct SlicePlan {
   int columns;
   int64_t chunk, chunks;
@@ -650,12 +653,13 @@ SlicePlan planSlices(const NormProblem &p, int vec, bool backward) {
   // them all
   const int64_t rows = p.ragged ? (p.rows + p.samples - 1) / p.samples : p.sample_rows;
   const int64_t turns = kSmallThreads / columns * (int64_t)kSmallTurns;
-  if (rows > turns || (p.ragged && p.rows > 16 * turns)) return plan;
+  if (rows > turns || (p.ragged && p.rows > 4 * turns)) return plan;
   // one round of blocks: 2,048 blocks for 256 samples of 64 rows of 128 channels took 74 us against 19 us for the three
   const int64_t slices = p.channels / (columns * vec), most = std::max<int64_t>(1, 2 * p.sm_count / slices);
   if (p.samples > most || (!p.ragged && rows <= kShortRows)) return plan;
   plan.columns = columns;
-  plan.chunk = backward && p.samples <= 4 ? p.samples : 1;  // backward, up to four: in one block, which writes the affine gradients
+  // backward, two rows a thread in all: one block for all samples, which then writes the affine gradients
+  plan.chunk = backward && p.samples <= 4 && p.rows <= turns / 2 ? p.samples : 1;
   plan.chunks = (p.samples + plan.chunk - 1) / plan.chunk;
   return plan;
 }
