@@ -632,7 +632,10 @@ double rowBytes(const NormProblem &p) {
 
 namespace {
 
-constexpr int kAffineSamples = 32;  // more: their sums are added up by a kernel of its own
+// More samples: their sums are added up by a kernel of its own.  Ragged samples of 64 half channels, gradients: 1,024 of 600
+// rows 143 us with it and 244 us in the input gradient kernel, whose first blocks walk down the samples; 128 of 5,000 rows
+// 101 and 98 us.
+constexpr int kAffineSamples = 256;
 
 // The one-launch form for samples of few rows: slices of `columns` vectors, `chunk` samples a block.  columns 0: it does
 // not apply.  Its blocks read 32 bytes or so of a row, and the chained launches of the other form cost about 9 us together.
