@@ -12,6 +12,8 @@
  * mlu_op.h:<line> (the reference's single public header) and the reference
  * implementation as <file>:<line> inside the reference tree.
  *
+ * Declarations marked "no counterpart in the reference" are extensions.
+ *
  * All pointers named *_desc and handle are host objects of this library.
  * All data pointers (indices, features, filters, workspace, outputs) are
  * device pointers, except indice_num[] of the two convolution functions,
