@@ -801,7 +801,7 @@ def _new(handle, like, shape, dtype):
     if _guards is not None:
         return _guards.empty(shape, dtype, like.device)
     if _on_own_queue(handle):
-        return like.new_empty(shape, dtype=dtype)
+        return like.new_empty(shape) if dtype == like.dtype else like.new_empty(shape, dtype=dtype)
     import torch
     current = torch.cuda.current_stream(handle.device)
     with torch.cuda.stream(torch.cuda.ExternalStream(handle.stream or 0, device=handle.device)):
