@@ -8,7 +8,7 @@ product with step_size and the two constants: 10 u of itself, and 4 u M / denomi
 step_size from m.  The parameter adds 3 u |p| (constant, product, difference) and its storage
 type's half step.  8 bits: half a step of e4m3 is 2^-4 of the value, 2^-10 of the scale below
 the normal range; a root raised to the smallest code is off by at most 2^-9 of the scale; the
-scale itself by 2 u.
+scale itself by 2 u and by what the block's largest value is off.
 """
 import pytest
 import torch
@@ -116,7 +116,9 @@ def check_step(ops, handle, sizes, dtype, grad_dtype, bits, seed, misalign=0, gs
             blocks = torch.zeros(-(-n // 256) * 256, dtype=torch.float64, device="cuda")
             blocks[:n] = want
             largest = blocks.view(-1, 256).abs().amax(1)
-            assert_within(scales, largest / 448.0, 1e-6 * largest, "scale %d" % i)
+            off = torch.zeros_like(blocks)
+            off[:n] = slack
+            assert_within(scales, largest / 448.0, (4 * U * largest + off.view(-1, 256).amax(1)) / 448.0, "scale %d" % i)
             per = scales.double().repeat_interleave(256)[:n]
             got = decode(codes, scales)
             assert_within(got, want, torch.maximum(2.0 ** -4 * want.abs(), tiny * per) * 1.001 + slack, "state %d" % i)
