@@ -215,7 +215,7 @@ cudaError_t dispatch(const NormProblem &p, Args... args) {
 ShortPlan planShort(const NormProblem &p, int vec) {
   ShortPlan plan{};
   const int group_channels = p.channels / p.groups;
-  if (p.ragged || p.sample_rows < 1 || p.sample_rows > kMostShortRows) return plan;
+  if (p.ragged || p.samples == 0 || p.sample_rows < 1 || p.sample_rows > kMostShortRows) return plan;
   if (p.sample_rows > kShortRows && p.samples < p.sample_rows * p.sample_rows / 4) return plan;
   plan.vec = group_channels % vec == 0 ? vec : 1;
   int lanes = 1;

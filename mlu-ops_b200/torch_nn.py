@@ -120,7 +120,8 @@ class AdamW(torch.optim.Optimizer):
     step count and the learning rate of each parameter group on the device, so that a captured step can be
     replayed (lr may then be a CUDA tensor; one step count for the whole group).  step(grad_scale=t)
     multiplies every gradient by the float32 CUDA tensor t of one element.  Before a step is captured, run one
-    outside of the capture: it allocates the states and the handles.
+    outside of the capture, which allocates the states and the handles, and let go of its loss: autograd cannot capture
+    a backward pass while an earlier graph of the same parameters is alive.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):

@@ -244,6 +244,19 @@ def test_constant_rows(ops, gpu_handle):
     assert not y.any() and (mean == 3).all() and torch.allclose(rstd, torch.full_like(rstd, EPS ** -0.5))
 
 
+@pytest.mark.parametrize("shape,ends", [((0, 5, 16), None), ((0, 16), None), ((3, 0, 16), None), ((0, 16), [0, 0]), ((0, 16), []),
+                                        ((40, 16), []), ((40, 16), [0, 0, 0])])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_nothing_to_normalise(ops, gpu_handle, guard_bands, shape, ends, dtype):
+    x, w, b, dy = make(shape, dtype, 30)
+    e = None if ends is None else torch.tensor(ends, dtype=torch.int32, device="cuda")
+    y, mean, rstd = ops.group_norm_act_forward(gpu_handle, x, w, b, 4, EPS, "silu", e)
+    dx, dw, db = ops.group_norm_act_backward(gpu_handle, dy, x, w, b, mean, rstd, 4, "silu", e)
+    assert mean.shape == ((shape[0] if ends is None else len(ends)), 4)
+    assert not y.any() and not dx.any() and not dw.any() and not db.any() and not mean.any()
+    assert torch.allclose(rstd, torch.full_like(rstd, EPS ** -0.5))
+
+
 def test_rows_without_a_sample_reach_nothing(ops, gpu_handle):
     """NaN and infinities behind the last sample change no output, and their own outputs are zero."""
     ends = torch.tensor([100, 250], dtype=torch.int32, device="cuda")
