@@ -97,6 +97,11 @@ struct Norm {
   // side in the forward pass, in both backward passes and in the formula evaluated step by step.
   __device__ __forceinline__ Two xhat(int j, Two x) const { return (x + minus_mean[UNIFORM ? 0 : j]) * rstd[UNIFORM ? 0 : j]; }
   __device__ __forceinline__ Two affine(int j, Two xh) const { return addRounded(xh * gamma[j], beta[j], one); }
+  // gamma du - m1 - xhat m2.  The product is rounded before m1 is taken off it, as it is in m1: in a group of one value
+  // nothing is left, where a fused difference would leave the rounding, which rstd makes 316 times larger.
+  __device__ __forceinline__ Two inputGrad(int j, Two du, Two xh, Two minus_m1, Two minus_m2) const {
+    return fma(xh, minus_m2, addRounded(du * gamma[j], minus_m1, one));
+  }
 };
 // value(c) for the channels of pair j of a thread whose first channel is `first`.
 template <int VEC, typename F>

@@ -391,7 +391,7 @@ inputGradKernel(const T *dy, const T *x, const void *weight, const void *bias, b
         const int q = UNIFORM ? 0 : j;
         const Two xh = c.xhat(j, v.pair(j));
         const Two du = activateGrad<ACT>(g.pair(j), c.affine(j, xh));
-        o[j] = fma(xh, minus_m2[q], fma(du, c.gamma[j], minus_m1[q])) * c.rstd[q];
+        o[j] = c.inputGrad(j, du, xh, minus_m1[q], minus_m2[q]) * c.rstd[q];
       }
       Values<T, VEC>::store(to, o);
     };
@@ -562,7 +562,7 @@ sliceKernel(const T *dy, const T *x, const void *weight, const void *bias, bool 
           const Two xh = c.xhat(j, v.pair(j));
           if (BACKWARD) {
             const Two du = activateGrad<ACT>(g.pair(j), c.affine(j, xh));
-            o[j] = fma(xh, minus_m2[q], fma(du, c.gamma[j], minus_m1[q])) * c.rstd[q];
+            o[j] = c.inputGrad(j, du, xh, minus_m1[q], minus_m2[q]) * c.rstd[q];
           } else {
             o[j] = activate<ACT>(c.affine(j, xh));
           }

@@ -157,7 +157,7 @@ shortSamplesKernel(const T *dy, const T *x, const void *weight, const void *bias
         const Two xh = c[k].xhat(0, v.pair(j));
         if (BACKWARD) {
           const Two du = activateGrad<ACT>(g.pair(j), c[k].affine(j, xh));
-          o[j] = fma(xh, minus_m2, fma(du, c[k].gamma[j], minus_m1)) * c[k].rstd[0];
+          o[j] = c[k].inputGrad(j, du, xh, minus_m1, minus_m2) * c[k].rstd[0];
         } else {
           o[j] = activate<ACT>(c[k].affine(j, xh));
         }

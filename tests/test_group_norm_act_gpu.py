@@ -257,6 +257,19 @@ def test_nothing_to_normalise(ops, gpu_handle, guard_bands, shape, ends, dtype):
     assert torch.allclose(rstd, torch.full_like(rstd, EPS ** -0.5))
 
 
+@pytest.mark.parametrize("shape,ends", [((50, 32), None), ((2, 32), [1, 2]), ((9, 32), [1, 2, 9]), ((600, 32), list(range(1, 601)))])
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+def test_a_group_of_one_value_has_no_input_gradient(ops, gpu_handle, shape, ends, act):
+    """The value is its own mean: the terms cancel exactly, nothing is left for rstd = 1 / sqrt(EPS) to enlarge."""
+    x, w, b, dy = make(shape, torch.float32, 31)
+    e = None if ends is None else torch.tensor(ends, dtype=torch.int32, device="cuda")
+    y, mean, rstd = ops.group_norm_act_forward(gpu_handle, x, w, b, 32, EPS, act, e)
+    dx, dw, db = ops.group_norm_act_backward(gpu_handle, dy, x, w, b, mean, rstd, 32, act, e)
+    ones = 2 if ends == [1, 2, 9] else shape[0]  # rows that are samples of their own
+    assert torch.equal(mean[:ones], x[:ones]) and not dx[:ones].any()
+    assert ones < shape[0] or not dw.any()
+
+
 def test_rows_without_a_sample_reach_nothing(ops, gpu_handle):
     """NaN and infinities behind the last sample change no output, and their own outputs are zero."""
     ends = torch.tensor([100, 250], dtype=torch.int32, device="cuda")
