@@ -162,11 +162,14 @@ class AdamW(torch.optim.Optimizer):
             known = self._plans[key] = (at, ops.MultiTensorAdamW(*tensors))
         return known[1]
 
+    def _new_schedule(self, index, group, device, step):
+        self._schedules[index] = (torch.full((), float(step), dtype=torch.float64, device=device),
+                                  torch.tensor([1.0, *group["betas"]], dtype=torch.float64, device=device))
+
     def _schedule(self, index, group, device):
         """Capturable: counts the group's step on the device and returns its schedule tensor."""
         if index not in self._schedules:
-            self._schedules[index] = (torch.zeros((), dtype=torch.float64, device=device),
-                                      torch.tensor([1.0, *group["betas"]], dtype=torch.float64, device=device))
+            self._new_schedule(index, group, device, 0)
         count, base = self._schedules[index]
         count += 1
         powers = 1.0 - base ** count
@@ -217,25 +220,61 @@ class AdamW(torch.optim.Optimizer):
         self._plans = {}
 
     def state_dict(self):
+        """As Optimizer.state_dict.  A capturable optimiser's step counts are read from the device, where replays count too."""
         out = super().state_dict()
-        out["schedules"] = {i: (c.clone(), b.clone()) for i, (c, b) in self._schedules.items()}
+        states = out["state"] = dict(out["state"])
+        for index, (count, _) in self._schedules.items():
+            for i in out["param_groups"][index]["params"]:
+                if i in states:
+                    states[i] = {**states[i], "step": int(count)}
         return out
 
+    def _loaded_state(self, p, state):
+        """A saved state of parameter `p` as this optimiser keeps it."""
+        out = {"step": int(state["step"])}
+        for key in ("exp_avg", "exp_avg_sq"):
+            value, numel = state[key], p.numel()
+            if self.state_bits == 32 and value.is_floating_point() and value.dtype != torch.float8_e4m3fn:
+                value = value.to(torch.float32)
+            elif self.state_bits == 32 or value.dtype not in (torch.uint8, torch.float8_e4m3fn):
+                raise ValueError("%s is %s, which is no state of %d bits" % (key, value.dtype, self.state_bits))
+            out[key] = value
+            if self.state_bits == 8:
+                out[key + "_scale"] = state[key + "_scale"].to(torch.float32)
+                if out[key + "_scale"].numel() != -(-numel // ops.SCALE_BLOCK):
+                    raise ValueError("%s has another number of scales" % key)
+            if value.numel() != numel:
+                raise ValueError("%s has %d elements, its parameter %d" % (key, value.numel(), numel))
+        return {key: v.detach().clone().to(p.device) if torch.is_tensor(v) else v for key, v in out.items()}
+
     def load_state_dict(self, state_dict):
-        """As Optimizer.load_state_dict, with the states in the types they were saved in (the base class would cast
-        them to the parameters')."""
+        """As Optimizer.load_state_dict, with the states in this class's types (the base class would cast them to the
+        parameters'); a state of torch.optim.AdamW is taken over.  Capturable: the parameters of a group must have
+        been saved at one step.  Graphs that were captured before update what was there before: capture again."""
         state_dict = dict(state_dict)
-        schedules = state_dict.pop("schedules", {})
+        counts = {i: int(pair[0]) for i, pair in state_dict.pop("schedules", {}).items()}  # (kept apart by earlier versions)
         if any(("exp_avg_scale" in s) != (self.state_bits == 8) for s in state_dict["state"].values()):
             raise ValueError("the saved states have another number of bits")
+        groups = state_dict["param_groups"]
+        for key in ("amsgrad", "maximize"):
+            if any(g.get(key) for g in groups):
+                raise ValueError("%s is not supported" % key)
+        params = dict(zip([i for g in groups for i in g["params"]], [p for g in self.param_groups for p in g["params"]]))
+        states = {i: self._loaded_state(params[i], s) for i, s in state_dict["state"].items() if i in params}
+        for index, g in enumerate(groups):
+            own = [states[i] for i in g["params"] if i in states]
+            for s in own:
+                s["step"] = counts.get(index, s["step"])
+            steps = {s["step"] for s in own}
+            if self.capturable and len(steps) > 1:
+                raise ValueError("capturable: one step count for a group, the saved ones are %s" % sorted(steps))
+            counts[index] = max(steps, default=counts.get(index, 0))
         super().load_state_dict(state_dict)
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(saved, params):
-            for key, value in state_dict["state"].get(i, {}).items():
-                self.state[p][key] = value.detach().clone().to(p.device) if torch.is_tensor(value) else value
-        self._schedules = {i: tuple(t.detach().clone() for t in pair) for i, pair in schedules.items()}
-        for i, pair in self._schedules.items():
-            device = self.param_groups[i]["params"][0].device
-            self._schedules[i] = tuple(t.to(device) for t in pair)
-        self._plans = {}
+        for i, s in states.items():
+            self.state[params[i]] = s
+        self._schedules, self._plans = {}, {}
+        for index, group in enumerate(self.param_groups):
+            if self.capturable and counts[index] and group["params"]:
+                self._new_schedule(index, group, group["params"][0].device, counts[index])
+            if not self.capturable and torch.is_tensor(group["lr"]):
+                group["lr"] = float(group["lr"])

@@ -1,0 +1,101 @@
+"""The optimiser's states on the GPU: what is saved after replayed graphs, and what the class keeps between steps.
+
+Tolerance against torch's optimiser: a step of 1e-2 has about 20 roundings of float (2^-24) of the value, as in
+test_torch_nn_gpu.py; the capturable schedule rounds its three floats once more.
+"""
+import importlib
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def nn_(pkg):
+    return importlib.import_module("mluops_b200.torch_nn")
+
+
+def parameters(seed=3):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(s, generator=gen, device="cuda")) for s in ((3, 3, 8, 16), (16,), (700, 33))]
+
+
+def set_grads(params, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    for p in params:
+        g = torch.randn(p.shape, generator=gen, device="cuda")
+        if p.grad is None:
+            p.grad = g
+        else:
+            p.grad.copy_(g)
+
+
+def copies(params):
+    return [torch.nn.Parameter(p.detach().clone()) for p in params]
+
+
+def capture(opt):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        opt.step()
+    return graph
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("second", [False, True])
+def test_resumes_after_replays(nn_, bits, second):
+    """Two eager steps, three replays, saved: three more steps elsewhere are those of an optimiser that ran eagerly."""
+    ours, plain = parameters(), parameters()
+    opt = nn_.AdamW(ours, lr=1e-2, state_bits=bits, capturable=True)
+    ref = nn_.AdamW(plain, lr=1e-2, state_bits=bits, capturable=second)
+    for step in range(2):
+        set_grads(ours, step)
+        set_grads(plain, step)
+        opt.step()
+        ref.step()
+    graph = capture(opt)
+    for step in range(2, 5):
+        set_grads(ours, step)
+        set_grads(plain, step)
+        graph.replay()
+        ref.step()
+    saved = opt.state_dict()
+    assert [s["step"] for s in saved["state"].values()] == [5, 5, 5]
+    more = copies(ours)
+    other = nn_.AdamW(more, lr=1e-2, state_bits=bits, capturable=second)
+    other.load_state_dict(saved)
+    for step in range(5, 8):
+        set_grads(more, step)
+        set_grads(plain, step)
+        other.step()
+        ref.step()
+    assert [s["step"] for s in other.state_dict()["state"].values()] == [8, 8, 8]
+    if bits == 32:
+        for p, q in zip(more, plain):
+            assert ((p - q).abs() <= 8 * 25 * 2.0 ** -24 * (1 + q.abs())).all()
+    elif second:  # the same arithmetic throughout
+        assert all(torch.equal(p, q) for p, q in zip(more, plain))
+
+
+def test_state_of_torchs_optimizer(nn_):
+    theirs = parameters()
+    ref = torch.optim.AdamW(theirs, lr=1e-2, foreach=False)
+    for step in range(4):
+        set_grads(theirs, step)
+        ref.step()
+    for capturable in (False, True):
+        ours, rest = copies(theirs), copies(theirs)
+        opt, base = nn_.AdamW(ours, lr=1e-2, capturable=capturable), torch.optim.AdamW(rest, lr=1e-2, foreach=False)
+        opt.load_state_dict(ref.state_dict())
+        base.load_state_dict(ref.state_dict())
+        for step in range(4, 7):
+            set_grads(ours, step)
+            set_grads(rest, step)
+            opt.step()
+            base.step()
+        for p, q in zip(ours, rest):
+            assert ((p - q).abs() <= 7 * 25 * 2.0 ** -24 * (1 + q.abs())).all()
+        assert len(opt._plans) == 1
