@@ -136,7 +136,7 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self.state_bits, self.capturable = state_bits, bool(capturable)
         self._plans = {}      # the tensors of each bucket, checked and laid out for the call
-        self._schedules = {}  # capturable: per group (step count, {lr, 1 - beta1^step, 1 - beta2^step})
+        self._schedules = {}  # capturable: per group (step count, {1, beta1, beta2}, the betas it holds)
 
     def _new_state(self, p):
         if self.state_bits == 32:
@@ -162,15 +162,20 @@ class AdamW(torch.optim.Optimizer):
             known = self._plans[key] = (at, ops.MultiTensorAdamW(*tensors))
         return known[1]
 
-    def _new_schedule(self, index, group, device, step):
-        self._schedules[index] = (torch.full((), float(step), dtype=torch.float64, device=device),
-                                  torch.tensor([1.0, *group["betas"]], dtype=torch.float64, device=device))
+    def _new_schedule(self, index, device, step):
+        self._schedules[index] = (torch.full((), float(step), dtype=torch.float64, device=device), None, None)
 
     def _schedule(self, index, group, device):
         """Capturable: counts the group's step on the device and returns its schedule tensor."""
         if index not in self._schedules:
-            self._new_schedule(index, group, device, 0)
-        count, base = self._schedules[index]
+            self._new_schedule(index, device, 0)
+        count, base, made_for = self._schedules[index]
+        betas = tuple(group["betas"])
+        if made_for != betas:
+            base = torch.ones(3, dtype=torch.float64, device=device)
+            base[1], base[2] = betas  # (filled on the device: nothing is copied from the host)
+            if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():  # what a graph fills is not kept for other calls
+                self._schedules[index] = (count, base, betas)
         count += 1
         powers = 1.0 - base ** count
         lr = group["lr"]
@@ -223,7 +228,7 @@ class AdamW(torch.optim.Optimizer):
         """As Optimizer.state_dict.  A capturable optimiser's step counts are read from the device, where replays count too."""
         out = super().state_dict()
         states = out["state"] = dict(out["state"])
-        for index, (count, _) in self._schedules.items():
+        for index, (count, *_) in self._schedules.items():
             for i in out["param_groups"][index]["params"]:
                 if i in states:
                     states[i] = {**states[i], "step": int(count)}
@@ -275,6 +280,6 @@ class AdamW(torch.optim.Optimizer):
         self._schedules, self._plans = {}, {}
         for index, group in enumerate(self.param_groups):
             if self.capturable and counts[index] and group["params"]:
-                self._new_schedule(index, group, group["params"][0].device, counts[index])
+                self._new_schedule(index, group["params"][0].device, counts[index])
             if not self.capturable and torch.is_tensor(group["lr"]):
                 group["lr"] = float(group["lr"])

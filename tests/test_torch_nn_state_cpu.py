@@ -174,3 +174,16 @@ def test_state_saved_with_its_counters_apart(nn_):
         other = nn_.AdamW(parameters(), lr=1e-2, capturable=capturable)
         other.load_state_dict(saved)
         assert [s["step"] for s in other.state_dict()["state"].values()] == [40, 40]
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_betas_that_change_between_steps(nn_, capturable):
+    ours, theirs = parameters(), parameters()
+    opt, ref = nn_.AdamW(ours, lr=1e-2, capturable=capturable), torch.optim.AdamW(theirs, lr=1e-2)
+    for step, betas in enumerate([(0.9, 0.999), (0.5, 0.9), (0.5, 0.9), (0.8, 0.99)]):
+        set_grads(ours, step)
+        set_grads(theirs, step)
+        opt.param_groups[0]["betas"] = ref.param_groups[0]["betas"] = betas
+        opt.step()
+        ref.step()
+    close(ours, theirs)

@@ -99,3 +99,22 @@ def test_state_of_torchs_optimizer(nn_):
         for p, q in zip(ours, rest):
             assert ((p - q).abs() <= 7 * 25 * 2.0 ** -24 * (1 + q.abs())).all()
         assert len(opt._plans) == 1
+
+
+def test_betas_that_change_between_steps(nn_):
+    """Eager and captured steps of a capturable optimiser use the betas of the moment, as the ordinary one does."""
+    sets = [parameters() for _ in range(3)]
+    opts = [nn_.AdamW(p, lr=1e-2, capturable=c) for p, c in zip(sets, (False, True, True))]
+    for step, betas in enumerate([(0.9, 0.999), (0.5, 0.9), (0.5, 0.9), (0.8, 0.99)]):
+        for i, (p, opt) in enumerate(zip(sets, opts)):
+            set_grads(p, step)
+            opt.param_groups[0]["betas"] = betas
+            if i == 2 and step:  # captured anew whenever they change, and back
+                if step != 2:
+                    graph = capture(opt)
+                graph.replay()
+            else:
+                opt.step()
+    for p, q, r in zip(*sets):
+        assert torch.equal(q, r)
+        assert ((p - q).abs() <= 4 * 25 * 2.0 ** -24 * (1 + p.abs())).all()
