@@ -810,6 +810,14 @@ def _new(handle, like, shape, dtype):
     return t
 
 
+def _written(t):
+    """Tells autograd that the library has written the caller's tensor: a backward pass that saved its old values then
+    refuses.  (Tensors of inference mode are not counted.)"""
+    import torch
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _spec(t):
     return None if t is None else (t.dtype, t.shape)
 
@@ -862,6 +870,8 @@ def group_norm_act_forward(handle, input, weight, bias, num_groups, epsilon=1e-5
                                         mean.data_ptr(), d_m, rstd.data_ptr())
     if st:
         check("mluOpGroupNormActForward", st)
+    if out is not None:
+        _written(out)
     return y, mean, rstd
 
 
@@ -882,6 +892,7 @@ def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd
     p_e = None if sample_ends is None else _address(handle, "sample_ends", sample_ends)
     p_m, p_r = _address(handle, "mean", mean), _address(handle, "rstd", rstd)
     num_groups = int(num_groups)
+    given = out is not None
     if out is None:
         out = torch.empty_like(input) if _on_own_queue(handle) else _new(handle, input, input.shape, input.dtype)
     p_o = _address(handle, "out", out)
@@ -908,6 +919,8 @@ def group_norm_act_backward(handle, output_grad, input, weight, bias, mean, rstd
                                          d_o, p_o, d_wg, p_wg, d_bg, p_bg)
     if st:
         check("mluOpGroupNormActBackward", st)
+    if given:
+        _written(out)
     return out, weight_grad, bias_grad
 
 
@@ -967,6 +980,9 @@ class MultiTensorAdamW:
         self._param_p, self._m_p, self._v_p = _addresses(self.params), _addresses(self.exp_avgs), _addresses(self.exp_avg_sqs)
         self._scale_p = [_addresses(v) for v in self.scales] or [None, None]
         self._numel_p = i64_array(self.numels)
+        # whose change autograd has to hear of: views share the count of their base (tensors of inference mode have none)
+        updated = [t for t in self.params + self.exp_avgs + self.exp_avg_sqs + sum(self.scales, []) if not t.is_inference()]
+        self._updated = list({id(t): t for t in (t._base if t._is_view() else t for t in updated)}.values())
 
     def step(self, handle, grads, lr, betas=(0.9, 0.999), epsilon=1e-8, weight_decay=0.01, step=1, grad_scale=None,
              schedule=None):
@@ -999,12 +1015,14 @@ class MultiTensorAdamW:
                                           self._m_p.buffer_info()[0], self._v_p.buffer_info()[0],
                                           *[p and p.buffer_info()[0] for p in self._scale_p], lr, betas[0], betas[1],
                                           epsilon, weight_decay, int(step), _ptr(grad_scale), _ptr(schedule)))
+        torch.autograd.graph.increment_version(self._updated)
 
 
 def _grouped_rows_call(name, handle, rows, weight, group_ends, columns, out):
     """The forward product and the input gradient: rows [R,K] times each group's matrix into [R, columns]."""
     p_x, p_w, p_e = (_address(handle, "the row matrix", rows), _address(handle, "weight", weight),
                      _address(handle, "group_ends", group_ends))
+    given = out is not None
     if out is None:
         out = _new(handle, rows, (rows.shape[0], columns), rows.dtype)
     p_y = _address(handle, "out", out)
@@ -1017,6 +1035,8 @@ def _grouped_rows_call(name, handle, rows, weight, group_ends, columns, out):
     st = getattr(lib(), name)(handle.ptr, d_x, p_x, d_w, p_w, d_e, p_e, d_y, p_y)
     if st:
         check(name, st)
+    if given:
+        _written(out)
     return out
 
 
@@ -1043,6 +1063,7 @@ def grouped_matmul_backward_weight(handle, input, output_grad, group_ends, dtype
     import torch
     p_x, p_g, p_e = (_address(handle, "input", input), _address(handle, "output_grad", output_grad),
                      _address(handle, "group_ends", group_ends))
+    given = out is not None
     if out is None:
         out = _new(handle, input, (group_ends.shape[0], input.shape[-1], output_grad.shape[-1]), dtype or input.dtype)
     p_w = _address(handle, "out", out)
@@ -1060,4 +1081,6 @@ def grouped_matmul_backward_weight(handle, input, output_grad, group_ends, dtype
                                                 plan.workspace, d_w, p_w)
     if st:
         check("mluOpGroupedMatMulBackwardWeight", st)
+    if given:
+        _written(out)
     return out
