@@ -118,7 +118,7 @@ class AdamW(torch.optim.Optimizer):
     and square root of the second in e4m3).  Parameters are dense CUDA tensors in float32, float16 or
     bfloat16; states are held in float or 8 bits whatever the parameter's type.  capturable=True keeps the
     step count and the learning rate of each parameter group on the device, so that a captured step can be
-    replayed (lr may then be a CUDA tensor; one step count for the whole group).  step(grad_scale=t)
+    replayed (lr may then be a CUDA tensor, a number is captured as it is; one step count for the whole group).  step(grad_scale=t)
     multiplies every gradient by the float32 CUDA tensor t of one element.  Before a step is captured, run one
     outside of the capture, which allocates the states and the handles, and let go of its loss: autograd cannot capture
     a backward pass while an earlier graph of the same parameters is alive.
@@ -173,13 +173,18 @@ class AdamW(torch.optim.Optimizer):
         betas = tuple(group["betas"])
         if made_for != betas:
             base = torch.ones(3, dtype=torch.float64, device=device)
-            base[1], base[2] = betas  # (filled on the device: nothing is copied from the host)
-            if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():  # what a graph fills is not kept for other calls
+            for i, beta in enumerate(betas):
+                base[i + 1].fill_(beta)  # (on the device: nothing is copied from the host, which a capture forbids)
+            # what a graph fills is not kept for other calls
+            if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
                 self._schedules[index] = (count, base, betas)
         count += 1
         powers = 1.0 - base ** count
         lr = group["lr"]
-        powers[0] = lr if torch.is_tensor(lr) else float(lr)
+        if torch.is_tensor(lr):
+            powers[0].copy_(lr)
+        else:
+            powers[0].fill_(float(lr))
         return powers.to(torch.float32)
 
     @torch.no_grad()

@@ -118,3 +118,19 @@ def test_betas_that_change_between_steps(nn_):
     for p, q, r in zip(*sets):
         assert torch.equal(q, r)
         assert ((p - q).abs() <= 4 * 25 * 2.0 ** -24 * (1 + p.abs())).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step_with_a_number_as_learning_rate(nn_, bits):
+    ours, plain = parameters(), parameters()
+    opt, ref = [nn_.AdamW(p, lr=1e-2, state_bits=bits, capturable=True) for p in (ours, plain)]
+    for p, o in ((ours, opt), (plain, ref)):
+        set_grads(p, 0)
+        o.step()
+    graph = capture(opt)
+    for step in (1, 2):
+        set_grads(ours, step)
+        set_grads(plain, step)
+        graph.replay()
+        ref.step()
+    assert all(torch.equal(p, q) for p, q in zip(ours, plain))
