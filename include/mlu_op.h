@@ -588,6 +588,12 @@ mluOpStatus_t MLUOP_WIN_API mluOpIndiceConvolutionForwardBuiltinWorkspace(
  *                element is code * scale, scale = largest magnitude of the 256 /
  *                448.  A square root that is not zero is never stored as zero.
  *                The update itself uses m and v before they are rounded.
+ *                Codes are the nearest ones here, which suits single steps: from
+ *                step to step a moment moves by less than half a step of its
+ *                code (sqrt(v) by 0.05 % at beta2 = 0.999, half a step is 3 to
+ *                6 %), so that over some thousand steps only the largest
+ *                element of a block of 256 follows its gradients.  For training use
+ *                mluOpMultiTensorAdamW_v2 with MLUOP_ADAMW_ROUND_STOCHASTIC.
  *                A block whose largest magnitude is below 1e-30 is stored as
  *                zeros with scale zero.
  *   schedule     NULL, or three device floats {lr, 1 - beta1^t, 1 - beta2^t} that
@@ -608,6 +614,31 @@ mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW(
     const double lr, const double beta1, const double beta2, const double epsilon,
     const double weight_decay, const int64_t step, const float *grad_scale,
     const float *schedule);
+
+/* How 8-bit states are rounded to their codes.  NEAREST: as above.  STOCHASTIC: to
+ * one of the two neighbouring codes, the nearer one the likelier, so that the
+ * stored value is right on average (to 2^-16 of a code's step) and follows the
+ * moments however little they move.  The choice depends on the step, the element's place in its tensor
+ * and the state only: a repeated call repeats it, however the tensors are spread
+ * over calls. */
+typedef enum {
+  MLUOP_ADAMW_ROUND_NEAREST = 0,
+  MLUOP_ADAMW_ROUND_STOCHASTIC = 1,
+} mluOpAdamWRounding_t;
+
+/* mluOpMultiTensorAdamW with the rounding of 8-bit states (float states are not
+ * affected).  step_count: NULL, or a device int64 that takes the place of step in
+ * that choice and is read when the kernels run; a schedule with 8-bit states and
+ * MLUOP_ADAMW_ROUND_STOCHASTIC needs it, since a replayed graph would repeat one
+ * choice otherwise. */
+mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW_v2(
+    mluOpHandle_t handle, const mluOpDataType_t param_dtype, const mluOpDataType_t grad_dtype,
+    const mluOpDataType_t state_dtype, const int64_t tensor_num, const int64_t element_num[],
+    void *const param[], const void *const grad[], void *const exp_avg[],
+    void *const exp_avg_sq[], float *const exp_avg_scale[], float *const exp_avg_sq_scale[],
+    const double lr, const double beta1, const double beta2, const double epsilon,
+    const double weight_decay, const int64_t step, const float *grad_scale,
+    const float *schedule, const mluOpAdamWRounding_t rounding, const int64_t *step_count);
 
 /* ------------------------------------- group norm with an activation */
 

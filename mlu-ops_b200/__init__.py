@@ -29,6 +29,8 @@ LAYOUT_NCHW, LAYOUT_NHWC, LAYOUT_HWCN, LAYOUT_NDHWC, LAYOUT_ARRAY, LAYOUT_NCDHW 
 # mluOpDataType_t
 DTYPE_INVALID, DTYPE_HALF, DTYPE_FLOAT, DTYPE_INT16, DTYPE_INT32, DTYPE_INT64 = 0, 1, 2, 4, 6, 9
 DTYPE_UINT8, DTYPE_BFLOAT16 = 7, 17
+# mluOpAdamWRounding_t
+ADAMW_ROUNDINGS = {"nearest": 0, "stochastic": 1}
 # mluOpGroupNormAct_t
 GROUP_NORM_ACTS = {"none": 0, "relu": 1, "silu": 2}
 
@@ -114,6 +116,7 @@ SIGNATURES = {
     "mluOpDynamicPointToVoxelBackward": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                                _vp, _szt, _vp, _vp]),
     "mluOpMultiTensorAdamW": (_int, [_vp, _int, _int, _int, _i64] + [_vp] * 7 + [ctypes.c_double] * 5 + [_i64, _vp, _vp]),
+    "mluOpMultiTensorAdamW_v2": (_int, [_vp, _int, _int, _int, _i64] + [_vp] * 7 + [ctypes.c_double] * 5 + [_i64, _vp, _vp, _int, _vp]),
     "mluOpGetGroupNormActForwardWorkspaceSize": (_int, [_vp, _vp, _vp, _i64, ctypes.POINTER(_szt)]),
     "mluOpGroupNormActForward": (_int, [_vp] * 9 + [_i64, ctypes.c_double, _int, _vp, _szt] + [_vp] * 6),
     "mluOpGetGroupNormActBackwardWorkspaceSize": (_int, [_vp, _vp, _vp, _i64, ctypes.POINTER(_szt)]),
@@ -985,14 +988,22 @@ class MultiTensorAdamW:
         self._updated = list({id(t): t for t in (t._base if t._is_view() else t for t in updated)}.values())
 
     def step(self, handle, grads, lr, betas=(0.9, 0.999), epsilon=1e-8, weight_decay=0.01, step=1, grad_scale=None,
-             schedule=None):
+             schedule=None, rounding="nearest", step_count=None):
         """One step with the gradients `grads` (dense, in the parameters' order; their type or float32).
 
         step counts from 1.  grad_scale: a float32 CUDA tensor of one element that every gradient is
         multiplied by (a clipping or loss-scale factor).  schedule: a float32 CUDA tensor {lr,
         1 - beta1^step, 1 - beta2^step} that takes the place of lr and step when the kernels run.
+
+        rounding of 8-bit states: "nearest", or "stochastic" for a training run, whose states stop following the
+        gradients when they are rounded to the nearest code at every step (mluOpMultiTensorAdamW_v2).  step_count: an
+        int64 CUDA tensor of one element that takes the place of step in the stochastic choice; a schedule needs it there.
         """
         import torch
+        if rounding not in ADAMW_ROUNDINGS:
+            raise ValueError("rounding is one of %s" % ", ".join(ADAMW_ROUNDINGS))
+        if rounding == "stochastic" and self.eight_bit and schedule is not None and step_count is None:
+            raise ValueError("stochastic rounding with a schedule needs a step_count")
         if len(grads) != len(self.params):
             raise ValueError("%d gradients for %d parameters" % (len(grads), len(self.params)))
         if not grads:
@@ -1007,14 +1018,19 @@ class MultiTensorAdamW:
             if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.get_device() != self.device
                                   or not t.is_contiguous()):
                 raise ValueError("%s is a dense float32 tensor of %d element(s) on the parameters' device" % (name, n))
+        if step_count is not None and (step_count.dtype != torch.int64 or step_count.numel() != 1
+                                       or step_count.get_device() != self.device):
+            raise ValueError("step_count is an int64 tensor of one element on the parameters' device")
         grad_p = _addresses(grads)
-        check("mluOpMultiTensorAdamW",
-              lib().mluOpMultiTensorAdamW(handle.ptr, _dtype_code(self.dtype), _dtype_code(dtype),
-                                          DTYPE_UINT8 if self.eight_bit else DTYPE_FLOAT, len(self.params),
-                                          self._numel_p, self._param_p.buffer_info()[0], grad_p.buffer_info()[0],
-                                          self._m_p.buffer_info()[0], self._v_p.buffer_info()[0],
-                                          *[p and p.buffer_info()[0] for p in self._scale_p], lr, betas[0], betas[1],
-                                          epsilon, weight_decay, int(step), _ptr(grad_scale), _ptr(schedule)))
+        args = (handle.ptr, _dtype_code(self.dtype), _dtype_code(dtype), DTYPE_UINT8 if self.eight_bit else DTYPE_FLOAT,
+                len(self.params), self._numel_p, self._param_p.buffer_info()[0], grad_p.buffer_info()[0],
+                self._m_p.buffer_info()[0], self._v_p.buffer_info()[0], *[p and p.buffer_info()[0] for p in self._scale_p],
+                lr, betas[0], betas[1], epsilon, weight_decay, int(step), _ptr(grad_scale), _ptr(schedule))
+        if rounding == "nearest":
+            check("mluOpMultiTensorAdamW", lib().mluOpMultiTensorAdamW(*args))
+        else:
+            check("mluOpMultiTensorAdamW_v2",
+                  lib().mluOpMultiTensorAdamW_v2(*args, ADAMW_ROUNDINGS[rounding], _ptr(step_count)))
         torch.autograd.graph.increment_version(self._updated)
 
 

@@ -1,4 +1,4 @@
-// mluOpMultiTensorAdamW: argument checks and dispatch.  No counterpart in the
+// mluOpMultiTensorAdamW and mluOpMultiTensorAdamW_v2: argument checks and dispatch.  No counterpart in the
 // reference with this shape (its kernels/adamw updates one tensor with float states).
 #include <cuda_runtime_api.h>
 
@@ -18,17 +18,13 @@ bool isParamType(mluOpDataType_t t) {
 
 bool aligned(const void *p, size_t to) { return reinterpret_cast<size_t>(p) % to == 0; }
 
-}  // namespace
-
-extern "C" {
-
-mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW(
-    mluOpHandle_t handle, const mluOpDataType_t param_dtype, const mluOpDataType_t grad_dtype,
-    const mluOpDataType_t state_dtype, const int64_t tensor_num, const int64_t element_num[], void *const param[],
-    const void *const grad[], void *const exp_avg[], void *const exp_avg_sq[], float *const exp_avg_scale[],
-    float *const exp_avg_sq_scale[], const double lr, const double beta1, const double beta2, const double epsilon,
-    const double weight_decay, const int64_t step, const float *grad_scale, const float *schedule) {
-  const std::string api = "[mluOpMultiTensorAdamW]";
+mluOpStatus_t runStep(const std::string &api, mluOpHandle_t handle, const mluOpDataType_t param_dtype,
+                      const mluOpDataType_t grad_dtype, const mluOpDataType_t state_dtype, const int64_t tensor_num,
+                      const int64_t element_num[], void *const param[], const void *const grad[],
+                      void *const exp_avg[], void *const exp_avg_sq[], float *const exp_avg_scale[],
+                      float *const exp_avg_sq_scale[], const double lr, const double beta1, const double beta2,
+                      const double epsilon, const double weight_decay, const int64_t step, const float *grad_scale,
+                      const float *schedule, const mluOpAdamWRounding_t rounding, const int64_t *step_count) {
   PARAM_CHECK(api, handle != nullptr);
   if (handle->arch < MLUOP_MLU370) {
     LOG(ERROR) << api << " needs a compute-capability 10.x device; this handle's device is not one.";
@@ -46,6 +42,10 @@ mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW(
   PARAM_CHECK(api, step >= 1);
   PARAM_CHECK(api, aligned(grad_scale, 4));
   PARAM_CHECK(api, aligned(schedule, 4));
+  PARAM_CHECK(api, aligned(step_count, 8));
+  PARAM_CHECK(api, rounding == MLUOP_ADAMW_ROUND_NEAREST || rounding == MLUOP_ADAMW_ROUND_STOCHASTIC);
+  const bool stochastic = rounding == MLUOP_ADAMW_ROUND_STOCHASTIC && state_dtype == MLUOP_DTYPE_UINT8;
+  PARAM_CHECK(api, !stochastic || schedule == nullptr || step_count != nullptr);
   if (tensor_num == 0) {
     VLOG(5) << api << " no tensors.";
     return MLUOP_STATUS_SUCCESS;
@@ -86,13 +86,41 @@ mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW(
   mluop::multi_tensor_adamw::AdamWProblem p{param_dtype, grad_dtype,    state_8bit,       tensor_num, element_num,
                                             param,       grad,          exp_avg,          exp_avg_sq, exp_avg_scale,
                                             exp_avg_sq_scale, lr,       beta1,            beta2,      epsilon,
-                                            weight_decay, step,         grad_scale,       schedule, handle->sm_count};
+                                            weight_decay, step,         grad_scale,       schedule, handle->sm_count,
+                                            stochastic,   step_count};
   const cudaError_t err = mluop::multi_tensor_adamw::launchMultiTensorAdamW(p, handle->queue);
   if (err != cudaSuccess) {
     LOG(ERROR) << api << " launch failed: " << cudaGetErrorString(err);
     return MLUOP_STATUS_EXECUTION_FAILED;
   }
   return MLUOP_STATUS_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" {
+
+mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW(
+    mluOpHandle_t handle, const mluOpDataType_t param_dtype, const mluOpDataType_t grad_dtype,
+    const mluOpDataType_t state_dtype, const int64_t tensor_num, const int64_t element_num[], void *const param[],
+    const void *const grad[], void *const exp_avg[], void *const exp_avg_sq[], float *const exp_avg_scale[],
+    float *const exp_avg_sq_scale[], const double lr, const double beta1, const double beta2, const double epsilon,
+    const double weight_decay, const int64_t step, const float *grad_scale, const float *schedule) {
+  return runStep("[mluOpMultiTensorAdamW]", handle, param_dtype, grad_dtype, state_dtype, tensor_num, element_num,
+                 param, grad, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, lr, beta1, beta2, epsilon,
+                 weight_decay, step, grad_scale, schedule, MLUOP_ADAMW_ROUND_NEAREST, nullptr);
+}
+
+mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW_v2(
+    mluOpHandle_t handle, const mluOpDataType_t param_dtype, const mluOpDataType_t grad_dtype,
+    const mluOpDataType_t state_dtype, const int64_t tensor_num, const int64_t element_num[], void *const param[],
+    const void *const grad[], void *const exp_avg[], void *const exp_avg_sq[], float *const exp_avg_scale[],
+    float *const exp_avg_sq_scale[], const double lr, const double beta1, const double beta2, const double epsilon,
+    const double weight_decay, const int64_t step, const float *grad_scale, const float *schedule,
+    const mluOpAdamWRounding_t rounding, const int64_t *step_count) {
+  return runStep("[mluOpMultiTensorAdamW_v2]", handle, param_dtype, grad_dtype, state_dtype, tensor_num, element_num,
+                 param, grad, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, lr, beta1, beta2, epsilon,
+                 weight_decay, step, grad_scale, schedule, rounding, step_count);
 }
 
 }  // extern "C"

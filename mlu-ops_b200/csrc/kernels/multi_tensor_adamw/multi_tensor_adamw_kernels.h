@@ -26,6 +26,8 @@ struct AdamWProblem {
   int64_t step;
   const float *grad_scale, *schedule;
   int sm_count;
+  bool stochastic;  // rounding of 8-bit states
+  const int64_t *step_count;
 };
 
 cudaError_t launchMultiTensorAdamW(const AdamWProblem &p, cudaStream_t stream);

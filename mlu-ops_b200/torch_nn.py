@@ -115,7 +115,8 @@ class AdamW(torch.optim.Optimizer):
     """AdamW with one launch for up to 480 tensors (mluOpMultiTensorAdamW).
 
     state_bits: 32, or 8 for states of one byte an element and one scale for 256 elements (first moment
-    and square root of the second in e4m3).  Parameters are dense CUDA tensors in float32, float16 or
+    and square root of the second in e4m3, rounded stochastically from the step and the element, so that small changes
+    of a moment are not lost; a resumed run repeats them).  Parameters are dense CUDA tensors in float32, float16 or
     bfloat16; states are held in float or 8 bits whatever the parameter's type.  capturable=True keeps the
     step count and the learning rate of each parameter group on the device, so that a captured step can be
     replayed (lr may then be a CUDA tensor, a number is captured as it is; one step count for the whole group).  step(grad_scale=t)
@@ -163,7 +164,7 @@ class AdamW(torch.optim.Optimizer):
         return known[1]
 
     def _new_schedule(self, index, device, step):
-        self._schedules[index] = (torch.full((), float(step), dtype=torch.float64, device=device), None, None)
+        self._schedules[index] = (torch.full((), step, dtype=torch.int64, device=device), None, None)
 
     def _schedule(self, index, group, device):
         """Capturable: counts the group's step on the device and returns its schedule tensor."""
@@ -216,6 +217,10 @@ class AdamW(torch.optim.Optimizer):
                             raise ValueError("capturable: the parameters of a group lie on one device")
                         schedules[device] = self._schedule(index, group, device)
                     more["schedule"] = schedules[device]
+                if self.state_bits == 8:
+                    more["rounding"] = "stochastic"
+                    if self.capturable:
+                        more["step_count"] = self._schedules[index][0]
                 lr = 0.0 if self.capturable else float(group["lr"])
                 plan.step(_handle(device), [p.grad.contiguous() for _, p in members], lr, group["betas"], group["eps"],
                           group["weight_decay"], max(count, 1), grad_scale=grad_scale, **more)
@@ -228,6 +233,7 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plans = {}
+        self._schedules = {i: (entry[0].to(torch.int64), None, None) for i, entry in self._schedules.items()}
 
     def state_dict(self):
         """As Optimizer.state_dict.  A capturable optimiser's step counts are read from the device, where replays count too."""
