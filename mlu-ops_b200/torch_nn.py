@@ -6,7 +6,8 @@ training step: group norm with an activation, products grouped by row blocks, th
     y = GroupedLinear(num_groups, 64, 128)(rows, ends)      # one matrix for each block of rows
     AdamW(model.parameters(), lr=1e-3, state_bits=8).step()
 
-Every tensor stays on the GPU and nothing is read back.  There is no CPU path.
+Every tensor stays on the GPU.  Nothing is read back, but for one check of the row order of a SparseConvTensor whose
+indices came from outside (SparseConvTensor.sample_ends).  There is no CPU path.
 """
 import math
 import sys
@@ -103,11 +104,10 @@ class GroupNormAct(nn.Module):
     def forward(self, x):
         if not isinstance(x, SparseConvTensor):
             return group_norm_act(x, self.num_groups, self.weight, self.bias, self.epsilon, self.activation)
-        ends = x.sample_ends()
         out = SparseConvTensor(group_norm_act(x.features, self.num_groups, self.weight, self.bias, self.epsilon,
-                                              self.activation, ends),
+                                              self.activation, x.sample_ends()),
                                x.indices, x.spatial_shape, x.batch_size, x.indice_dict)
-        out._sample_ends = ends
+        out._ends = x._ends
         return out
 
 

@@ -51,7 +51,7 @@ def _triple(v):
 class Rulebook:
     """What mluOpGetIndicePairs produced for one geometry (shared through indice_key)."""
     __slots__ = ("indice_pairs", "out_indices", "indice_num", "num_act_out", "out_space", "filter_space", "sub_m",
-                 "shared", "table", "input_table")
+                 "shared", "table", "input_table", "ends")
 
     def forward_table(self, handle):
         """The neighbour table of a rulebook that several layers share (an indice_key), built at its
@@ -73,6 +73,39 @@ class Rulebook:
         return self.input_table
 
 
+class _SampleEnds:
+    """Where the samples of an `indices` tensor end, worked out once for all that share it: a tensor, what a norm or a
+    submanifold layer makes of it, the rulebook.  ordered: the indices, if they are in ascending order by construction."""
+
+    def __init__(self, ordered=None):
+        self.made = None
+        self.ordered = None if ordered is None else (ordered, self._version(ordered))
+
+    @staticmethod
+    def _version(indices):
+        return None if indices.is_inference() else indices._version  # (inference mode does not count writes in place)
+
+    def of(self, indices, batch_size):
+        state = (indices, self._version(indices))
+
+        def same(known):
+            return known is not None and known[0] is indices and known[1] == state[1]
+
+        if same(self.made) and self.made[2] == batch_size:
+            return self.made[3]
+        capturing = torch.cuda.is_current_stream_capturing()
+        batch = indices[:, 0].contiguous()
+        if not same(self.ordered):
+            if capturing:
+                raise RuntimeError("the sample ends of this tensor are not known yet: call sample_ends() before the capture")
+            if batch.numel() and bool((batch[1:] < batch[:-1]).any() | (batch[0] < 0) | (batch[-1] >= batch_size)):
+                raise ValueError("the rows are not in ascending order of their batch index")
+        ends = torch.searchsorted(batch, torch.arange(1, batch_size + 1, dtype=torch.int32, device=batch.device), out_int32=True)
+        if not capturing:  # (what a graph computes is not there before it is replayed)
+            self.made = (*state, batch_size, ends)
+        return ends
+
+
 class SparseConvTensor:
     """features [N,C] and int32 indices [N,4] = (batch, z, y, x) of the active voxels of a
     batch of grids of size spatial_shape = (D, H, W).  Rows must not repeat a coordinate."""
@@ -85,18 +118,14 @@ class SparseConvTensor:
         self.spatial_shape = [int(v) for v in spatial_shape]
         self.batch_size = int(batch_size)
         self.indice_dict = {} if indice_dict is None else indice_dict
+        self._ends = _SampleEnds()
 
     def sample_ends(self):
         """int32 [batch_size] on the device: where each sample's rows end, for operators that work sample by sample.  The
-        rows must lie in ascending order of the batch index (one host read at the first call; kept with the tensor)."""
-        ends = getattr(self, "_sample_ends", None)
-        if ends is None:
-            batch = self.indices[:, 0].contiguous()
-            if batch.numel() and bool((batch[1:] < batch[:-1]).any() | (batch[0] < 0) | (batch[-1] >= self.batch_size)):
-                raise ValueError("the rows are not in ascending order of their batch index")
-            ends = torch.searchsorted(batch, torch.arange(1, self.batch_size + 1, dtype=torch.int32, device=batch.device))
-            self._sample_ends = ends = ends.to(torch.int32)
-        return ends
+        rows must lie in ascending order of the batch index.  That takes one host read for indices that came from
+        outside; those of a strided layer are in order, and submanifold layers and norms hand on what is known.  Kept until
+        the indices are replaced or written in place (writes in place under inference mode are not seen)."""
+        return self._ends.of(self.indices, self.batch_size)
 
     def dense(self):
         """[batch, C, D, H, W] with zeros where no voxel is active."""
@@ -185,6 +214,7 @@ class SparseConvolution(nn.Module):
         rb.indice_num = num.cpu().tolist()  # the convolution API takes the counts as a host array
         rb.num_act_out, rb.out_space = n_out, out_space
         rb.filter_space, rb.sub_m = list(self.kernel_size), int(self.subm)
+        rb.ends = x._ends if self.subm else _SampleEnds(ordered=rb.out_indices)
         rb.shared = self.indice_key is not None  # other layers will come for it: worth keeping its tables
         if self.indice_key is not None:
             x.indice_dict[self.indice_key] = rb
@@ -195,7 +225,9 @@ class SparseConvolution(nn.Module):
         out = _IndiceConvFunction.apply(x.features, self.weight, rb)
         if self.bias is not None:
             out = out + self.bias
-        return SparseConvTensor(out, rb.out_indices, rb.out_space, x.batch_size, x.indice_dict)
+        y = SparseConvTensor(out, rb.out_indices, rb.out_space, x.batch_size, x.indice_dict)
+        y._ends = getattr(rb, "ends", None) or y._ends
+        return y
 
 
 class SparseConv3d(SparseConvolution):
