@@ -667,8 +667,8 @@ typedef enum {
  * [N, num_groups] FLOAT, outputs (an empty sample: mean 0, rstd 1 / sqrt(epsilon)).
  * epsilon > 0 in float.  Statistics are held in float and combined in a fixed order:
  * results are reproducible run to run.  Descriptors are contiguous, every tensor
- * has fewer than 2^31 rows and C <= 65536.  output may be input (in place), else it
- * may not overlap it (refused).
+ * has fewer than 2^31 rows and C <= 65536.  output may be input (in place); else
+ * outputs and workspace may overlap no other tensor of the call (refused).
  * The workspace query may answer 0; workspace may be NULL then.  Samples of one size
  * may be as short and as many as they like; of samples with sample_ends there should
  * be no more than some hundreds, since a block joins its sums at the end of each.
@@ -703,8 +703,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpGetGroupNormActBackwardWorkspaceSize(
  * at 0 is 0.  input_grad has the input's type; weight_grad and bias_grad [C]
  * FLOAT or the input's type, both NULL (descriptors too) to leave them out.
  * input_grad rows of no sample are zero, and no such row reaches a sum.
- * input_grad may be output_grad or input (in place), else it may not overlap them
- * (refused). */
+ * input_grad may be output_grad or input (in place); else outputs and workspace may
+ * overlap no other tensor of the call (refused). */
 mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActBackward(
     mluOpHandle_t handle, const mluOpTensorDescriptor_t output_grad_desc,
     const void *output_grad, const mluOpTensorDescriptor_t input_desc, const void *input,
@@ -730,10 +730,11 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActBackward(
  * is read back, and a captured graph follows them.  Entries of group_ends are
  * clamped to [previous entry, rows]; groups may be empty; rows from the last
  * entry on belong to no group and their outputs are zero.  1 <= G <= 1024, rows <
- * 2^31, 1 <= Ci, Co <= 65536, and fewer than 2^30 tiles of 128 x 64 results.  HALF and BFLOAT16 run on the tensor cores where Ci
- * and Co are multiples of 8 and the three pointers are 16-byte aligned, else on the
- * general kernel.  Outputs may not overlap inputs (refused).  Results are reproducible run
- * to run.  Asynchronous on the handle's queue; no workspace. */
+ * 2^31, 1 <= Ci, Co <= 65536, and fewer than 2^30 tiles of 128 x 64 results.  HALF
+ * and BFLOAT16 run on the tensor cores where Ci and Co are multiples of 8 and the
+ * three pointers are 16-byte aligned, else on the general kernel.  Outputs and
+ * workspace may overlap no other tensor (refused).  Results are reproducible run to
+ * run.  Asynchronous on the handle's queue; no workspace. */
 mluOpStatus_t MLUOP_WIN_API mluOpGroupedMatMulForward(
     mluOpHandle_t handle, const mluOpTensorDescriptor_t input_desc, const void *input,
     const mluOpTensorDescriptor_t weight_desc, const void *weight,

@@ -11,6 +11,7 @@
 #include "core/tensor.h"
 #include "kernels/group_norm_act/group_norm_act_kernels.h"
 
+using mluop::Span;
 using mluop::group_norm_act::NormProblem;
 
 namespace {
@@ -214,6 +215,10 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActForward(
     if (sample_ends_desc != nullptr) PARAM_CHECK(api, sample_ends != nullptr && aligned(sample_ends, 4));
   }
   RETURN_UNLESS_OK(workspaceCheck(api, p, false, workspace, workspace_size));
+  const Span ws(workspace, workspace_size), w(weight_desc, weight), b(bias_desc, bias), ends(sample_ends_desc, sample_ends);
+  // (output on input: checked above)
+  PARAM_CHECK(api, mluop::writtenApart({{output_desc, output}, {mean_desc, mean}, {rstd_desc, rstd}, ws}, {w, b, ends}));
+  PARAM_CHECK(api, mluop::writtenApart({{mean_desc, mean}, {rstd_desc, rstd}, ws}, {{input_desc, input}}));
   if (handle->host_only) {
     LOG(ERROR) << api << " this handle was created without a CUDA device; nothing can be launched.";
     return MLUOP_STATUS_EXECUTION_FAILED;
@@ -283,6 +288,12 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupNormActBackward(
     if (sample_ends_desc != nullptr) PARAM_CHECK(api, sample_ends != nullptr && aligned(sample_ends, 4));
   }
   RETURN_UNLESS_OK(workspaceCheck(api, p, true, workspace, workspace_size));
+  const Span ws(workspace, workspace_size), w(weight_desc, weight), b(bias_desc, bias), ends(sample_ends_desc, sample_ends);
+  const Span dw(weight_grad_desc, weight_grad), db(bias_grad_desc, bias_grad);
+  // (input_grad on output_grad or input: checked above)
+  PARAM_CHECK(api, mluop::writtenApart({{input_grad_desc, input_grad}, dw, db, ws},
+                                       {w, b, ends, {mean_desc, mean}, {rstd_desc, rstd}}));
+  PARAM_CHECK(api, mluop::writtenApart({dw, db, ws}, {{output_grad_desc, output_grad}, {input_desc, input}}));
   if (handle->host_only) {
     LOG(ERROR) << api << " this handle was created without a CUDA device; nothing can be launched.";
     return MLUOP_STATUS_EXECUTION_FAILED;

@@ -2,9 +2,7 @@
 // argument checks and dispatch.  No counterpart in the reference.
 #include <cuda_runtime_api.h>
 
-#include <initializer_list>
 #include <string>
-#include <utility>
 
 #include "core/context.h"
 #include "core/logging.h"
@@ -85,15 +83,6 @@ mluOpStatus_t endsCheck(const std::string &api, const Problem &p, const mluOpTen
   return MLUOP_STATUS_SUCCESS;
 }
 
-// Whether the output lies on none of the inputs.
-bool apart(const mluOpTensorDescriptor_t desc, const void *out,
-           std::initializer_list<std::pair<mluOpTensorDescriptor_t, const void *>> inputs) {
-  const size_t bytes = mluop::denseBytes(desc);
-  for (const auto &in : inputs)
-    if (mluop::overlap(out, bytes, in.second, mluop::denseBytes(in.first))) return false;
-  return true;
-}
-
 mluOpStatus_t run(const std::string &api, mluOpHandle_t handle, Problem &p, const void *a, const void *b,
                   const void *ends, void *c, void *workspace) {
   if (handle->host_only) {
@@ -148,7 +137,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupedMatMulForward(mluOpHandle_t handle, cons
   PARAM_CHECK(api, weight != nullptr && aligned(weight, p.dtype));
   PARAM_CHECK(api, group_ends != nullptr && aligned(group_ends, MLUOP_DTYPE_INT32));
   PARAM_CHECK(api, output != nullptr && aligned(output, p.dtype));
-  PARAM_CHECK(api, apart(output_desc, output, {{input_desc, input}, {weight_desc, weight}, {group_ends_desc, group_ends}}));
+  PARAM_CHECK(api, mluop::writtenApart({{output_desc, output}},
+                                       {{input_desc, input}, {weight_desc, weight}, {group_ends_desc, group_ends}}));
   return run(api, handle, p, input, weight, group_ends, output, nullptr);
 }
 
@@ -174,8 +164,9 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupedMatMulBackwardInput(
   PARAM_CHECK(api, weight != nullptr && aligned(weight, p.dtype));
   PARAM_CHECK(api, group_ends != nullptr && aligned(group_ends, MLUOP_DTYPE_INT32));
   PARAM_CHECK(api, input_grad != nullptr && aligned(input_grad, p.dtype));
-  PARAM_CHECK(api, apart(input_grad_desc, input_grad,
-                         {{output_grad_desc, output_grad}, {weight_desc, weight}, {group_ends_desc, group_ends}}));
+  PARAM_CHECK(api, mluop::writtenApart({{input_grad_desc, input_grad}}, {{output_grad_desc, output_grad},
+                                                                         {weight_desc, weight},
+                                                                         {group_ends_desc, group_ends}}));
   return run(api, handle, p, output_grad, weight, group_ends, input_grad, nullptr);
 }
 
@@ -215,8 +206,6 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupedMatMulBackwardWeight(
     PARAM_CHECK(api, input != nullptr && aligned(input, p.dtype));
     PARAM_CHECK(api, output_grad != nullptr && aligned(output_grad, p.dtype));
     PARAM_CHECK(api, group_ends != nullptr && aligned(group_ends, MLUOP_DTYPE_INT32));
-    PARAM_CHECK(api, apart(weight_grad_desc, weight_grad,
-                           {{input_desc, input}, {output_grad_desc, output_grad}, {group_ends_desc, group_ends}}));
   }
   const size_t need = mluop::grouped_matmul::weightGradWorkspaceBytes(p);
   if (workspace == nullptr || workspace_size < need) {
@@ -224,6 +213,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpGroupedMatMulBackwardWeight(
                << " bytes mluOpGetGroupedMatMulBackwardWeightWorkspaceSize reports.";
     return MLUOP_STATUS_BAD_PARAM;
   }
+  PARAM_CHECK(api, mluop::writtenApart({{weight_grad_desc, weight_grad}, {workspace, workspace_size}},
+                                       {{input_desc, input}, {output_grad_desc, output_grad}, {group_ends_desc, group_ends}}));
   if (p.rows == 0 && !handle->host_only) {  // every group is empty
     mluop::DeviceGuard guard(handle);
     const size_t bytes = (size_t)mluOpGetTensorElementNum(weight_grad_desc) *
