@@ -936,11 +936,27 @@ def _addresses(tensors):
     return array.array("Q", map(torch.Tensor.data_ptr, tensors))
 
 
+def same_order(a, b):
+    """Whether tensors a and b are dense and have their elements in the same order in memory."""
+    if a.is_contiguous() and b.is_contiguous():
+        return a.numel() == b.numel()
+    if a.shape != b.shape:
+        return False
+    expected = 1
+    for stride, other, size in sorted(zip(a.stride(), b.stride(), a.shape)):
+        if size != 1:
+            if stride != expected or other != expected:
+                return False
+            expected *= size
+    return True
+
+
 class MultiTensorAdamW:
     """AdamW steps over the same tensors through mluOpMultiTensorAdamW.
 
     params: dense CUDA tensors of one type (float32, float16 or bfloat16), updated in place;
-    exp_avgs and exp_avg_sqs: their states, of the same element counts.  float32 states hold the
+    exp_avgs and exp_avg_sqs: their states, of the same element counts; a parameter that is not
+    contiguous (channels last, say) has states and gradients of its shape and strides.  float32 states hold the
     moments themselves.  8-bit states (uint8 or float8_e4m3fn) hold the first moment and the
     square root of the second as e4m3 codes; exp_avg_scales and exp_avg_sq_scales then hold one
     float32 for each 256 elements of their tensor (code * scale is the value).  The object keeps
@@ -966,16 +982,20 @@ class MultiTensorAdamW:
                 raise ValueError("parameters have one type, states are float32, or 8 bits with scales")
             if m.numel() != n or v.numel() != n:
                 raise ValueError("a state has another number of elements than its parameter")
+            if not (same_order(p, p) and same_order(p, m) and same_order(p, v)):
+                raise ValueError("every tensor is dense, and a state laid out like its parameter")
             spans += [p, m, v]
         for scales in self.scales:
             for q, n in zip(scales, self.numels):
                 if q.dtype != torch.float32 or q.numel() != -(-n // SCALE_BLOCK):
                     raise ValueError("scales are float32, one for each %d elements" % SCALE_BLOCK)
+                if not q.is_contiguous():
+                    raise ValueError("every tensor is dense")
                 spans.append(q)
         end = 0
         for begin, size, t in sorted(((t.data_ptr(), t.numel() * t.element_size(), t) for t in spans),
                                      key=lambda x: x[:2]):
-            if t.get_device() != self.device or not t.is_contiguous():
+            if t.get_device() != self.device:
                 raise ValueError("every tensor is dense and on the same device")
             if size and begin < end:
                 raise ValueError("two of the tensors overlap")
@@ -983,6 +1003,7 @@ class MultiTensorAdamW:
         self._param_p, self._m_p, self._v_p = _addresses(self.params), _addresses(self.exp_avgs), _addresses(self.exp_avg_sqs)
         self._scale_p = [_addresses(v) for v in self.scales] or [None, None]
         self._numel_p = i64_array(self.numels)
+        self._contiguous = all(p.is_contiguous() for p in self.params)
         # whose change autograd has to hear of: views share the count of their base (tensors of inference mode have none)
         updated = [t for t in self.params + self.exp_avgs + self.exp_avg_sqs + sum(self.scales, []) if not t.is_inference()]
         self._updated = list({id(t): t for t in (t._base if t._is_view() else t for t in updated)}.values())
@@ -1012,8 +1033,9 @@ class MultiTensorAdamW:
             raise ValueError("the tensors lie on device %s, the handle on CUDA device %d" % (self.device, handle.device))
         dtype, of = grads[0].dtype, torch.Tensor  # (mapped methods: a step of many small tensors is mostly this)
         if (list(map(of.numel, grads)) != self.numels or {g.dtype for g in grads} != {dtype}
-                or set(map(of.get_device, grads)) != {self.device} or not all(map(of.is_contiguous, grads))):
-            raise ValueError("gradients are dense, of one type, on the parameters' device and of their sizes")
+                or set(map(of.get_device, grads)) != {self.device}
+                or not (all(map(of.is_contiguous, grads)) if self._contiguous else all(map(same_order, self.params, grads)))):
+            raise ValueError("gradients are dense, of one type, on the parameters' device and of their sizes and order")
         for name, t, n in (("grad_scale", grad_scale, 1), ("schedule", schedule, 3)):
             if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.get_device() != self.device
                                   or not t.is_contiguous()):

@@ -115,10 +115,11 @@ class AdamW(torch.optim.Optimizer):
     """AdamW with one launch for up to 480 tensors (mluOpMultiTensorAdamW).
 
     state_bits: 32, or 8 for states of one byte an element and one scale for 256 elements (first moment
-    and square root of the second in e4m3, rounded stochastically from the step and the element, so that small changes
-    of a moment are not lost; a resumed run repeats them).  Parameters are dense CUDA tensors in float32, float16 or
-    bfloat16; states are held in float or 8 bits whatever the parameter's type.  capturable=True keeps the
-    step count and the learning rate of each parameter group on the device, so that a captured step can be
+    and square root of the second in e4m3, rounded stochastically from the step and the element, so that
+    small changes of a moment are not lost; a resumed run repeats them).  Parameters are dense CUDA tensors, in
+    any order of dimensions, in float32, float16 or bfloat16; states are held in float or 8 bits whatever the
+    parameter's type.  capturable=True keeps the step count and the learning rate of each parameter group on the
+    device, so that a captured step can be
     replayed (lr may then be a CUDA tensor, a number is captured as it is; one step count for the whole group).  step(grad_scale=t)
     multiplies every gradient by the float32 CUDA tensor t of one element.  Before a step is captured, run one
     outside of the capture, which allocates the states and the handles, and let go of its loss: autograd cannot capture
@@ -140,22 +141,26 @@ class AdamW(torch.optim.Optimizer):
         self._schedules = {}  # capturable: per group (step count, {1, beta1, beta2}, the betas it holds)
 
     def _new_state(self, p):
-        if self.state_bits == 32:
-            zeros = [torch.zeros(p.numel(), dtype=torch.float32, device=p.device) for _ in range(2)]
-            return {"step": 0, "exp_avg": zeros[0].view(p.shape), "exp_avg_sq": zeros[1].view(p.shape)}
-        blocks = -(-p.numel() // ops.SCALE_BLOCK)
         state = {"step": 0}
-        for key in ("exp_avg", "exp_avg_sq"):
-            state[key] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
-            state[key + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        for key in ("exp_avg", "exp_avg_sq"):  # (in the parameter's order)
+            state[key] = torch.zeros_like(p, dtype=torch.float32 if self.state_bits == 32 else torch.uint8, requires_grad=False)
+            if self.state_bits == 8:
+                state[key + "_scale"] = torch.zeros(-(-p.numel() // ops.SCALE_BLOCK), dtype=torch.float32, device=p.device)
         return state
+
+    @staticmethod
+    def _gradient(p):
+        """The gradient in the parameter's order."""
+        if p.is_contiguous():
+            return p.grad.contiguous()
+        return p.grad if ops.same_order(p, p.grad) else torch.empty_like(p, dtype=p.grad.dtype).copy_(p.grad)
 
     def _bucket(self, key, params):
         """The plan for these parameters, built anew where a parameter or state lies elsewhere than before."""
         states = [self.state[p] for p in params]
         keys = ["exp_avg", "exp_avg_sq"] + (["exp_avg_scale", "exp_avg_sq_scale"] if self.state_bits == 8 else [])
         tensors = [params] + [[s[k] for s in states] for k in keys]
-        at = [list(map(torch.Tensor.data_ptr, v)) for v in tensors]
+        at = [list(map(torch.Tensor.data_ptr, v)) for v in tensors] + [p.is_contiguous() or p.stride() for p in params]
         known = self._plans.get(key)
         if known is None or known[0] != at:
             if len(self._plans) >= 64:  # the set of parameters that have gradients changes from step to step
@@ -222,7 +227,7 @@ class AdamW(torch.optim.Optimizer):
                     if self.capturable:
                         more["step_count"] = self._schedules[index][0]
                 lr = 0.0 if self.capturable else float(group["lr"])
-                plan.step(_handle(device), [p.grad.contiguous() for _, p in members], lr, group["betas"], group["eps"],
+                plan.step(_handle(device), [self._gradient(p) for _, p in members], lr, group["betas"], group["eps"],
                           group["weight_decay"], max(count, 1), grad_scale=grad_scale, **more)
         return loss
 
@@ -254,13 +259,17 @@ class AdamW(torch.optim.Optimizer):
                 value = value.to(torch.float32)
             elif self.state_bits == 32 or value.dtype not in (torch.uint8, torch.float8_e4m3fn):
                 raise ValueError("%s is %s, which is no state of %d bits" % (key, value.dtype, self.state_bits))
+            if value.numel() != numel:
+                raise ValueError("%s has %d elements, its parameter %d" % (key, value.numel(), numel))
+            if not ops.same_order(p, value):
+                if self.state_bits == 8:
+                    raise ValueError("8-bit states lie in the order that their parameter had in memory")
+                value = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(value.reshape(p.shape))
             out[key] = value
             if self.state_bits == 8:
                 out[key + "_scale"] = state[key + "_scale"].to(torch.float32)
                 if out[key + "_scale"].numel() != -(-numel // ops.SCALE_BLOCK):
                     raise ValueError("%s has another number of scales" % key)
-            if value.numel() != numel:
-                raise ValueError("%s has %d elements, its parameter %d" % (key, value.numel(), numel))
         return {key: v.detach().clone().to(p.device) if torch.is_tensor(v) else v for key, v in out.items()}
 
     def load_state_dict(self, state_dict):
