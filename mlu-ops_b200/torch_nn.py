@@ -199,6 +199,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        calls = []  # every refusal comes before the first update
         for index, group in enumerate(self.param_groups):
             buckets = {}
             for i, p in enumerate(group["params"]):
@@ -209,26 +210,29 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     state.update(self._new_state(p))
-                state["step"] += 1
-                count = 0 if self.capturable else state["step"]
+                count = 0 if self.capturable else state["step"] + 1
                 buckets.setdefault((p.device, p.dtype, p.grad.dtype, count), []).append((i, p))
-            schedules = {}
+            if self.capturable and len({key[0] for key in buckets}) > 1:
+                raise ValueError("capturable: the parameters of a group lie on one device")
             for (device, dtype, grad_dtype, count), members in buckets.items():
                 plan = self._bucket((index, device, dtype, grad_dtype, tuple(i for i, _ in members)), [p for _, p in members])
-                more = {}
+                calls.append((index, group, device, count, plan, [p for _, p in members]))
+        schedules = {}
+        for index, group, device, count, plan, members in calls:
+            more = {}
+            if self.capturable:
+                if index not in schedules:
+                    schedules[index] = self._schedule(index, group, device)
+                more["schedule"] = schedules[index]
+            if self.state_bits == 8:
+                more["rounding"] = "stochastic"
                 if self.capturable:
-                    if device not in schedules:
-                        if schedules:
-                            raise ValueError("capturable: the parameters of a group lie on one device")
-                        schedules[device] = self._schedule(index, group, device)
-                    more["schedule"] = schedules[device]
-                if self.state_bits == 8:
-                    more["rounding"] = "stochastic"
-                    if self.capturable:
-                        more["step_count"] = self._schedules[index][0]
-                lr = 0.0 if self.capturable else float(group["lr"])
-                plan.step(_handle(device), [self._gradient(p) for _, p in members], lr, group["betas"], group["eps"],
-                          group["weight_decay"], max(count, 1), grad_scale=grad_scale, **more)
+                    more["step_count"] = self._schedules[index][0]
+            lr = 0.0 if self.capturable else float(group["lr"])
+            plan.step(_handle(device), list(map(self._gradient, members)), lr, group["betas"], group["eps"],
+                      group["weight_decay"], max(count, 1), grad_scale=grad_scale, **more)
+            for p in members:
+                self.state[p]["step"] += 1
         return loss
 
     def __getstate__(self):  # (copies and pickles; what is laid out for the calls is not part of it)

@@ -187,3 +187,26 @@ def test_betas_that_change_between_steps(nn_, capturable):
         opt.step()
         ref.step()
     close(ours, theirs)
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_changes_nothing(nn_, capturable):
+    """A gradient that is refused, in the second group: no parameter of either group moves, and no step is counted."""
+    ours, theirs = parameters(), parameters()
+    odd = torch.nn.Parameter(torch.zeros(3, 2, dtype=torch.float64))
+    opt = nn_.AdamW([{"params": ours}, {"params": [odd]}], lr=1e-2, capturable=capturable)
+    ref = torch.optim.AdamW(theirs, lr=1e-2)
+    for step in range(3):
+        set_grads(ours, step)
+        set_grads(theirs, step)
+        if step == 1:
+            before = [p.detach().clone() for p in ours]
+            odd.grad = torch.sparse_coo_tensor([[0]], [[1.0, 1.0]], (3, 2), dtype=torch.float64)
+            with pytest.raises(ValueError, match="sparse"):
+                opt.step()
+            assert all(torch.equal(p, q) for p, q in zip(ours, before))
+            odd.grad = None
+        opt.step()
+        ref.step()
+    close(ours, theirs)
+    assert [s["step"] for s in opt.state_dict()["state"].values()][:2] == [3, 3]
