@@ -66,27 +66,36 @@ def build(force=False, verbose=False):
     flags += os.environ.get("MLUOP_B200_NVCC_FLAGS", "").split()  # extra compiler flags (experiments)
 
     # One object per source, compiled side by side; an object is kept while its own source, every
-    # header and the flags are older than it.
+    # header and the flags are older than it.  What a build that fails or is cut off leaves behind is
+    # not taken for more: outputs get their names when they are whole, and the flags' file says
+    # nothing while objects of other flags come in.
     flag_file = os.path.join(OBJ_DIR, "flags.txt")
     same_flags = os.path.isfile(flag_file) and open(flag_file).read() == " ".join([nvcc] + flags)
+    if not same_flags and os.path.isfile(flag_file):
+        os.remove(flag_file)
     newest_header = max(os.path.getmtime(p) for p in headers())
+
+    def run(out, cmd):
+        part = os.path.join(os.path.dirname(out), "part." + os.path.basename(out))
+        subprocess.check_call([nvcc, "-o", part] + cmd)
+        os.replace(part, out)
 
     def compile_one(src):
         obj = os.path.join(OBJ_DIR, os.path.relpath(src, CSRC).replace(os.sep, "__") + ".o")
         if (force or not same_flags or not os.path.isfile(obj)
                 or os.path.getmtime(obj) < max(os.path.getmtime(src), newest_header)):
-            cmd = [nvcc, "-c", "-o", obj] + flags + [src]
+            cmd = ["-c"] + flags + [src]
             if verbose:
-                print(" ".join(cmd))
-            subprocess.check_call(cmd)
+                print(" ".join([nvcc] + cmd))
+            run(obj, cmd)
         return obj
 
     with concurrent.futures.ThreadPoolExecutor(os.cpu_count()) as pool:
         objects = list(pool.map(compile_one, sources()))
     with open(flag_file, "w") as f:
         f.write(" ".join([nvcc] + flags))
-    subprocess.check_call([nvcc, "-shared", "-o", LIB, "-gencode", "arch=compute_100a,code=sm_100a"] + objects
-                          + ["-lcudart_static", "-lpthread", "-ldl", "-lrt"])
+    run(LIB, ["-shared", "-gencode", "arch=compute_100a,code=sm_100a"] + objects
+        + ["-lcudart_static", "-lpthread", "-ldl", "-lrt"])
     return LIB
 
 
