@@ -217,6 +217,9 @@ class AdamW(torch.optim.Optimizer):
             for (device, dtype, grad_dtype, count), members in buckets.items():
                 plan = self._bucket((index, device, dtype, grad_dtype, tuple(i for i, _ in members)), [p for _, p in members])
                 calls.append((index, group, device, count, plan, [p for _, p in members]))
+        if (not self.capturable and any(device.type == "cuda" for _, _, device, *_ in calls)
+                and torch.cuda.is_current_stream_capturing()):
+            raise RuntimeError("capturable=True is needed to capture a step: a graph would repeat this one's count and rate")
         schedules = {}
         for index, group, device, count, plan, members in calls:
             more = {}

@@ -134,3 +134,23 @@ def test_captured_step_with_a_number_as_learning_rate(nn_, bits):
         graph.replay()
         ref.step()
     assert all(torch.equal(p, q) for p, q in zip(ours, plain))
+
+
+def test_capture_of_an_ordinary_step_is_refused(nn_):
+    """Its step count and learning rate would be those of the capture in every replay."""
+    ours = parameters()
+    opt = nn_.AdamW(ours, lr=1e-2)
+    set_grads(ours, 0)
+    opt.step()
+    before = [p.detach().clone() for p in ours]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    one = torch.zeros(1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(RuntimeError, match="capturable=True"):
+            opt.step()
+        one += 1
+    graph.replay()
+    assert one.item() == 1 and all(torch.equal(p, q) for p, q in zip(ours, before))
+    assert [s["step"] for s in opt.state.values()] == [1, 1, 1]
