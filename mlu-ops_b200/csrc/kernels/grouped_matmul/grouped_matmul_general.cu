@@ -285,9 +285,12 @@ WeightGradPlan planWeightGrad(const Problem &p, bool tensor_cores) {
   const int64_t blocks = (tensor_cores ? 1 : 4) * (int64_t)p.sm_count * kM / plan.tile_m;
   int64_t chunk = (p.rows * tiles + 4 * blocks - 1) / (4 * blocks);
   chunk = (std::max<int64_t>(chunk, 512) + 63) / 64 * 64;
-  // Several groups of a thousand rows or less on average: one unit each.  (13 groups of 4,999 rows, 200 x 328: 8 us for the
-  // largest group's products against 13 us and the second kernel's 10 us.)
-  if (p.groups >= 4 && p.rows <= 8192) chunk = (std::max<int64_t>(p.rows, 1) + 63) / 64 * 64;
+  // Tensor cores, eight groups or more of a thousand rows or less on average: one unit each, which saves the second kernel.
+  // 8,192 rows in half, unsplit and split, groups of one size | sizes from a log-normal of 1.2 | all rows in one group, us:
+  // 13 groups of 200 x 328 15 and 31 | 16 and 24 | 46 and 25; 16 of 64 x 64 10 and 12 | 14 and 16 | 45 and 14; 4 of 64 x 64,
+  // which are split, 18 and 15 | 25 and 15 | 45 and 15.  The general kernel's step is ten times as long: in float, 13 of
+  // 64 x 64 42 and 43 | 104 and 41 | 482 and 39.
+  if (tensor_cores && p.groups >= 8 && p.rows <= 8192) chunk = (std::max<int64_t>(p.rows, 1) + 63) / 64 * 64;
   plan.chunk_rows = chunk;
   plan.slots = p.rows > chunk ? 2 * p.rows / chunk : 0;  // ceil(r / chunk) <= 2 r / chunk for the groups that are split
   plan.maps = 0;
