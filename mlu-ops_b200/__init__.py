@@ -982,7 +982,8 @@ class MultiTensorAdamW:
                 raise ValueError("parameters have one type, states are float32, or 8 bits with scales")
             if m.numel() != n or v.numel() != n:
                 raise ValueError("a state has another number of elements than its parameter")
-            if not (same_order(p, p) and same_order(p, m) and same_order(p, v)):
+            if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()
+                    or same_order(p, p) and same_order(p, m) and same_order(p, v)):
                 raise ValueError("every tensor is dense, and a state laid out like its parameter")
             spans += [p, m, v]
         for scales in self.scales:

@@ -52,8 +52,9 @@ __device__ __forceinline__ void storeAffineGrad(void *p, bool is_float, int c, d
   else static_cast<T *>(p)[c] = fromFloat<T>((float)v);
 }
 
-// 1 / (1 + exp(-u)).  The approximations are good to 2^-22, and flush what is below the float range, where the quotient
-// is 0 or 1 in float.
+// 1 / (1 + exp(-u)).  The approximations are good to 2^-22 of their results; the rounding of u log2(e) before them puts
+// exp(-u) off by |u| 2^-24 of itself (2^-17 at u = -80, which is 2^-17 of a sigmoid of 10^-35; for positive u it vanishes
+// beside the 1).  They flush what is below the float range, where the quotient is 0 or 1 in float.
 __device__ __forceinline__ Two sigmoid(Two u) {
   float2 e = split(u * two(-1.4426950408889634f, -1.4426950408889634f));
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
