@@ -592,8 +592,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpIndiceConvolutionForwardBuiltinWorkspace(
  *                step to step a moment moves by less than half a step of its
  *                code (sqrt(v) by 0.05 % at beta2 = 0.999, half a step is 3 to
  *                6 %), so that over some thousand steps only the largest
- *                element of a block of 256 follows its gradients.  For training use
- *                mluOpMultiTensorAdamW_v2 with MLUOP_ADAMW_ROUND_STOCHASTIC.
+ *                element of a block of 256 follows its gradients.  For training
+ *                use mluOpMultiTensorAdamW_v2 with MLUOP_ADAMW_ROUND_STOCHASTIC.
  *                A block whose largest magnitude is below 1e-30 is stored as
  *                zeros with scale zero.
  *   schedule     NULL, or three device floats {lr, 1 - beta1^t, 1 - beta2^t} that
@@ -618,9 +618,9 @@ mluOpStatus_t MLUOP_WIN_API mluOpMultiTensorAdamW(
 /* How 8-bit states are rounded to their codes.  NEAREST: as above.  STOCHASTIC: to
  * one of the two neighbouring codes, the nearer one the likelier, so that the
  * stored value is right on average (to 2^-16 of a code's step) and follows the
- * moments however little they move.  The choice depends on the step, the element's place in its tensor
- * and the state only: a repeated call repeats it, however the tensors are spread
- * over calls. */
+ * moments however little they move.  The choice depends on the step, the element's
+ * place in its tensor and the state only: a repeated call repeats it, however the
+ * tensors are spread over calls. */
 typedef enum {
   MLUOP_ADAMW_ROUND_NEAREST = 0,
   MLUOP_ADAMW_ROUND_STOCHASTIC = 1,
