@@ -168,12 +168,18 @@ class AdamW(torch.optim.Optimizer):
             known = self._plans[key] = (at, ops.MultiTensorAdamW(*tensors))
         return known[1]
 
+    @staticmethod
+    def _refuse_capture(device):
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("run one step before the capture: replays would clear states that the graph makes")
+
     def _new_schedule(self, index, device, step):
         self._schedules[index] = (torch.full((), step, dtype=torch.int64, device=device), None, None)
 
     def _schedule(self, index, group, device):
         """Capturable: counts the group's step on the device and returns its schedule tensor."""
         if index not in self._schedules:
+            self._refuse_capture(device)
             self._new_schedule(index, device, 0)
         count, base, made_for = self._schedules[index]
         betas = tuple(group["betas"])
@@ -209,6 +215,7 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("sparse gradients are not supported")
                 state = self.state[p]
                 if not state:
+                    self._refuse_capture(p.device)
                     state.update(self._new_state(p))
                 count = 0 if self.capturable else state["step"] + 1
                 buckets.setdefault((p.device, p.dtype, p.grad.dtype, count), []).append((i, p))

@@ -154,3 +154,31 @@ def test_capture_of_an_ordinary_step_is_refused(nn_):
     graph.replay()
     assert one.item() == 1 and all(torch.equal(p, q) for p, q in zip(ours, before))
     assert [s["step"] for s in opt.state.values()] == [1, 1, 1]
+
+
+@pytest.mark.parametrize("loaded", [False, True])
+def test_capture_of_the_first_step_is_refused(nn_, loaded):
+    """States and counts made inside a graph would be cleared by every replay.  (loaded: states without a step yet.)"""
+    ours = parameters()
+    opt = nn_.AdamW(ours, lr=1e-2, capturable=True)
+    set_grads(ours, 0)
+    if loaded:
+        first = nn_.AdamW(copies(ours), lr=1e-2, capturable=True)
+        for p in first.param_groups[0]["params"]:
+            first.state[p] = first._new_state(p)
+        opt.load_state_dict(first.state_dict())
+    before = [p.detach().clone() for p in ours]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    one = torch.zeros(1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            opt.step()
+        one += 1
+    graph.replay()
+    assert one.item() == 1 and all(torch.equal(p, q) for p, q in zip(ours, before))
+    opt.step()
+    graph = capture(opt)
+    graph.replay()
+    assert [s["step"] for s in opt.state_dict()["state"].values()] == [2, 2, 2]
