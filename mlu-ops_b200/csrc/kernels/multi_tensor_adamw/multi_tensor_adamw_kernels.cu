@@ -45,6 +45,8 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "core/convert.cuh"
@@ -475,6 +477,9 @@ cudaError_t launchAll(const AdamWProblem &p, cudaStream_t stream) {
   t.c.beta2 = (float)p.beta2;
   t.c.one_minus_beta2 = (float)(1.0 - p.beta2);
   t.c.epsilon = (float)p.epsilon;
+  // The 8-bit step's reciprocal takes denormals for zero: an element without a gradient would become 0 * infinity.  A root
+  // that is not zero is above 2^-75, so that nothing else can tell.
+  if (p.state_8bit && p.epsilon > 0.0) t.c.epsilon = std::max(t.c.epsilon, FLT_MIN);
   t.c.one = 1.0f;
   t.c.decay = (float)(1.0 - p.lr * p.weight_decay);
   t.c.step_size = (float)(p.lr / (1.0 - std::pow(p.beta1, (double)p.step)));

@@ -188,3 +188,18 @@ def test_states_follow_gradients_that_change(pkg, factor):
     ratio = decode(state["exp_avg_sq"], state["exp_avg_sq_scale"]) / v.double().sqrt()
     for half in (ratio[::2], ratio[1::2]):
         assert abs(float(half.median()) - 1) <= 0.045, float(half.median())
+
+
+@pytest.mark.parametrize("rounding", ["nearest", "stochastic"])
+@pytest.mark.parametrize("epsilon", [1e-30, 1e-39, 1e-42])
+def test_small_epsilons(ops, gpu_handle, rounding, epsilon):
+    """Elements without a gradient: 0 / epsilon = 0 for every epsilon that a float holds, denormal ones among them."""
+    for misalign in (0, 1):
+        state = make([2048 + 100], misalign=misalign)
+        state[1][0].zero_()
+        for t in state[2] + state[3] + state[4] + state[5]:
+            t.zero_()
+        before = state[0][0].clone()
+        p, g, m, v, ms, vs = state
+        ops.MultiTensorAdamW(p, m, v, ms, vs).step(gpu_handle, g, 1e-3, epsilon=epsilon, weight_decay=0.0, rounding=rounding)
+        assert torch.equal(p[0], before)
